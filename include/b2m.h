@@ -70,6 +70,7 @@ typedef int32_t b2m_status;
 #define B2M_INT32 6
 #define B2M_INT64 7
 #define B2M_FLOAT16 10
+#define B2M_FLOAT8E4M3FN 17 /* codes of an 8-bit KV cache only */
 
 /* Arithmetic modes for the floating-point ops. */
 #define B2M_MODE_EXACT 0 /* bitwise identical to the reference Dart kernels */
@@ -512,6 +513,94 @@ B2M_API b2m_status b2m_rotary_dev(b2m_ctx *ctx, const float *x, int64_t x_rs, co
                                   int32_t pos_per_batch, const float *cos_cache, const float *sin_cache,
                                   int32_t half, int32_t max_pos, float *y, int64_t y_rs, int32_t b, int32_t s,
                                   int32_t heads, int32_t head_dim, int32_t rotary_dim, int32_t interleaved);
+
+/* ---- 8-bit KV cache ------------------------------------------------------
+ * A quantised form of b2m_gqa_dev's cache for serving: half the bytes of an
+ * f16 cache and a quarter of the fp32 one's. A row (one position of one kv
+ * head, head_dim values x) is head_dim codes of one byte and an fp32 scale:
+ *   scale = fl32(max|x| / M),  code = round-half-even(x / scale),
+ *   value = fl32(code * scale),
+ * with M = 127 (type B2M_INT8) or 448 (B2M_FLOAT8E4M3FN). x is what
+ * GroupQueryAttention caches (keys after the head norm and rotary), formed
+ * without intermediate rounding. A row of zeros has scale 0; a row with a
+ * value that is not finite is stored with a NaN scale and zero codes: it reads
+ * back as NaN, and only queries that see it get NaN. No counterpart in the
+ * reference, whose cache is float32 (lib/src/onnx_ops.dart:1844).
+ *
+ * One layer's cache: codes [b][kvh][cap][head_dim] (4-byte aligned), scales
+ * [b][kvh][cap], device memory owned by the caller. head_dim <= 256. */
+typedef struct b2m_kv8_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int32_t type; /* B2M_INT8 or B2M_FLOAT8E4M3FN */
+  int32_t b, kvh, cap, head_dim;
+} b2m_kv8_cache;
+
+/* Quantises s new tokens per sequence into positions past[b] .. past[b]+s-1.
+ * k / v: [b][s] rows of kvh*head_dim floats (row stride kv_rs). k_gain: NULL,
+ * or the keys' head-norm gains [kvh][head_dim] (as the k rows of
+ * b2m_gqa_qknorm_dev's qk_gain) with epsilon eps. depth: NULL (token i sits at
+ * position past + i), or [b][s] int32: rotary position past + depth[i], for
+ * drafted trees (0 <= depth[i] < s). cos / sin: [cap][rotary_half] or NULL.
+ * A token past the capacity is not written and raises the capacity error; a
+ * negative past or a depth outside [0, s) is an index error and writes
+ * nothing for that token (reported by the next synchronising call). */
+B2M_API b2m_status b2m_kv8_append_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const float *k, const float *v,
+                                      int64_t kv_rs, const float *k_gain, double eps, const int32_t *past,
+                                      const int32_t *depth, const float *cos_cache, const float *sin_cache,
+                                      int32_t rotary_half, int32_t rotary_dim, int32_t interleaved, int32_t s);
+
+/* Values of the n positions from start[b] (int32 device memory; NULL: from 0)
+ * as fp32: k_out / v_out [b][kvh][n][head_dim], either may be NULL. A position
+ * outside [0, cap) is an index error and leaves its row as it was. */
+B2M_API b2m_status b2m_kv8_read_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const int32_t *start, int32_t n,
+                                    float *k_out, float *v_out);
+
+/* GroupQueryAttention over the 8-bit cache: b2m_kv8_append_dev of the call's
+ * tokens, then softmax(scale * q . K^T) . V on the cached values, arguments as
+ * b2m_gqa_dev / b2m_gqa_qknorm_dev. qk_gain: NULL, or [h + kvh][head_dim] head
+ * norm gains of q and k (q and k themselves are not modified). tree: NULL for
+ * causal attention (token i sees positions 0 .. past + i), or [b][s] uint64
+ * with s <= 64 and depth given: token i sees every cached position below past
+ * and the new tokens j whose bit j is set (a token sees itself only if its
+ * own bit is set; one that sees nothing gets zeros). out: [b][s] rows of
+ * h*head_dim, and / or out16, the same rounded to f16 (h*head_dim % 8 == 0);
+ * one of them may be NULL. Scale <= 0 means 1/sqrt(head_dim). fp32 rows carry
+ * fp32 accuracy (operands split into two f16 terms on the tensor cores);
+ * with out16 alone, q and the softmax weights are rounded to f16, below the
+ * output's own rounding. EXACT attention mode (b2m_set_attention_mode) runs
+ * the fp32 CUDA-core kernel. */
+B2M_API b2m_status b2m_gqa_kv8_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const float *q, const float *k,
+                                   const float *v, int64_t q_rs, int64_t kv_rs, const float *qk_gain, double eps,
+                                   const int32_t *past, const uint64_t *tree, const int32_t *depth,
+                                   const float *cos_cache, const float *sin_cache, int32_t rotary_half,
+                                   int32_t rotary_dim, int32_t interleaved, float *out, uint16_t *out16, int32_t s,
+                                   int32_t h, float scale);
+
+/* Keeps the accepted path of a drafted tree: rows past[b] + path[b][j] of
+ * every head move to past[b] + j for j < count[b] (path: [b][n] int32, strictly
+ * increasing, path[j] < n; count: [b], 0 .. n; device memory). The rows behind
+ * them stay as they are. `layers` caches laid out one behind another (codes
+ * [layers][b][kvh][cap][head_dim], scales alike) move in one launch. A
+ * sequence with a bad path, count or past moves nothing and raises the index
+ * error. past itself is not changed. */
+B2M_API b2m_status b2m_kv8_keep_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, int32_t layers, const int32_t *past,
+                                    const int32_t *path, const int32_t *count, int32_t n);
+
+/* Log probabilities over rows of v logits (row stride ld >= v, v < 2^31):
+ *   logprob[r] = x[ids[r]] - ln sum e^x   (ids and logprob both given or NULL),
+ *   entropy[r] = -sum p ln p               (nats; may be NULL),
+ *   top_ids[r][0..k) = the k largest logits' ids, largest first, equal logits
+ *   by the lowest id; top_logprobs [r][k] their log probabilities (may be
+ *   NULL). 0 <= k <= 32, k <= v. -inf logits have probability 0. A row with a
+ * NaN or +inf logit, or with -inf only, has no distribution: its log
+ * probabilities and entropy are NaN (top_ids still go by the logits, NaN
+ * last). An id outside [0, v) is an index error and gives NaN. Next to
+ * b2m_argmax_dev; no counterpart in the reference. */
+#define B2M_LOGPROBS_MAX_K 32
+B2M_API b2m_status b2m_logprobs_dev(b2m_ctx *ctx, const float *logits, int64_t ld, const int64_t *ids, int64_t rows,
+                                    int64_t v, float *logprob, float *entropy, int32_t k, int64_t *top_ids,
+                                    float *top_logprobs);
 
 /* past[i] += delta for i < n (int32 device counters of a decode loop). */
 B2M_API b2m_status b2m_advance_positions_dev(b2m_ctx *ctx, int32_t *past, int32_t n, int32_t delta);

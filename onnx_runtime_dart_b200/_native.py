@@ -31,6 +31,7 @@ B2M_INT8 = 3
 B2M_INT32 = 6
 B2M_INT64 = 7
 B2M_FLOAT16 = 10
+B2M_FLOAT8E4M3FN = 17
 
 MODE_EXACT = 0
 MODE_FAST = 1
@@ -39,6 +40,7 @@ ROUTE_GEMV, ROUTE_TC_F16, ROUTE_OTHER = 0, 1, 2  # b2m_matmul_nbits_route
 
 MAX_RANK = 8
 NOALLOC_SCRATCH_BYTES = 8 << 20
+LOGPROBS_MAX_K = 32
 
 
 class B2mError(RuntimeError):
@@ -100,6 +102,16 @@ _f32 = ctypes.c_float
 _vp = ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _i32p = ctypes.POINTER(ctypes.c_int32)
+
+
+class Kv8Cache(ctypes.Structure):
+    """b2m_kv8_cache: one layer's 8-bit KV cache (device pointers, shape)."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("type", _i32), ("b", _i32),
+                ("kvh", _i32), ("cap", _i32), ("head_dim", _i32)]
+
+
+_kv8p = ctypes.POINTER(Kv8Cache)
 
 # name -> (restype, argtypes); the full export list of include/b2m.h.
 SIGNATURES = {
@@ -180,6 +192,13 @@ SIGNATURES = {
     "b2m_dynamic_quantize_linear_dev": (_i32, [_c_ctx, _vp, _i64, _vp, _vp, _vp]),
     "b2m_rotary_dev": (_i32, [_c_ctx, _vp, _i64, _vp, _i32, _vp, _vp, _i32, _i32, _vp, _i64, _i32, _i32, _i32,
                               _i32, _i32, _i32]),
+    "b2m_kv8_append_dev": (_i32, [_c_ctx, _kv8p, _vp, _vp, _i64, _vp, ctypes.c_double, _vp, _vp, _vp, _vp, _i32, _i32,
+                                  _i32, _i32]),
+    "b2m_kv8_read_dev": (_i32, [_c_ctx, _kv8p, _vp, _i32, _vp, _vp]),
+    "b2m_gqa_kv8_dev": (_i32, [_c_ctx, _kv8p, _vp, _vp, _vp, _i64, _i64, _vp, ctypes.c_double, _vp, _vp, _vp, _vp,
+                               _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _f32]),
+    "b2m_kv8_keep_dev": (_i32, [_c_ctx, _kv8p, _i32, _vp, _vp, _vp, _i32]),
+    "b2m_logprobs_dev": (_i32, [_c_ctx, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _vp, _vp]),
     "b2m_advance_positions_dev": (_i32, [_c_ctx, _vp, _i32, _i32]),
     "b2m_weight_export": (_i32, [_c_weight, _vp, ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)]),
     "b2m_weight_import": (_i32, [_c_ctx, _vp, ctypes.c_size_t, ctypes.POINTER(_c_weight)]),

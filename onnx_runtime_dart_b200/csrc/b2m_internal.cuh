@@ -425,6 +425,43 @@ void launch_rotary(const float *x, int64_t x_rs, const int64_t *pos, int pos_per
                    const float *sin, int half, int max_pos, float *y, int64_t y_rs, int B, int S, int heads, int D,
                    int rot, int interleaved, int32_t *err, cudaStream_t s);
 
+// 8-bit KV cache (k_kv8.cu): one layer's codes [B][KVH][CAP][D] and scales
+// [B][KVH][CAP], and the call's new tokens.
+struct Kv8Args {
+  uint8_t *kc = nullptr, *vc = nullptr;
+  float *ks = nullptr, *vs = nullptr;
+  bool e4m3 = false;  // e4m3 codes, else int8
+  int B = 0, KVH = 0, CAP = 0, D = 0;
+  const int32_t *past = nullptr;
+  // New tokens: [B][S] rows.
+  int S = 0, H = 0;
+  const float *q = nullptr, *k = nullptr, *v = nullptr;
+  int64_t q_rs = 0, kv_rs = 0;
+  const float *q_gain = nullptr, *k_gain = nullptr;  // [H][D] / [KVH][D] head norm gains, or null
+  double eps = 0.0;
+  // A drafted tree: bit j of tree[b][i] says that token i sees token j;
+  // depth[b][i] its distance from the root. Null: a causal run of tokens.
+  const uint64_t *tree = nullptr;
+  const int32_t *depth = nullptr;
+  const float *cos = nullptr, *sin = nullptr;  // [CAP][half] or null
+  int half = 0, rot = 0, interleaved = 0;
+  float scale = 1.f;
+  float *out = nullptr;     // [B][S][H*D], either may be null
+  __half *out16 = nullptr;
+  int32_t *err = nullptr;
+};
+void launch_kv8_append(const Kv8Args &a, cudaStream_t s);
+void launch_kv8_read(const Kv8Args &a, const int32_t *start, int n, float *k_out, float *v_out, cudaStream_t s);
+void launch_kv8_keep(const Kv8Args &a, int layers, const int32_t *path, const int32_t *count, int n, cudaStream_t s);
+// Appends the call's keys and values, then attends. `exact`: the fp32
+// CUDA-core kernel only.
+void launch_kv8_attend(const Kv8Args &a, bool exact, cudaStream_t s);
+
+// Log probabilities (k_logprobs.cu). ids / logprob, entropy, and top_ids /
+// top_lp (k > 0) may be null as their entry point says.
+void launch_logprobs(const float *x, int64_t ld, const int64_t *ids, int64_t rows, int64_t V, float *logprob,
+                     float *entropy, int k, int64_t *top_ids, float *top_lp, int32_t *err, cudaStream_t s);
+
 // DynamicQuantizeLinear (k_quant.cu): y = quantized x, scale / zp written to
 // device memory. `partial` holds dql_partial_floats() floats; `counter` is a
 // zeroed device word the kernel leaves zeroed.

@@ -1,0 +1,355 @@
+// 8-bit KV cache: quantised append, read-back, attention over the cache and
+// the move of accepted rows.
+//
+// A cached row (one position of one kv head, D values) is stored as D codes of
+// one byte and one fp32 scale:
+//   s = fl32(max|x| / M),  code = round-half-even(x / s),  value = code * s,
+// M = 127 for int8 codes and 448 for e4m3 codes. x is the real-number result
+// of the head norm and rotary on the fp32 inputs: it is formed in double, so
+// the code is the right one also next to a rounding border. A row with a
+// value that is not finite gets a NaN scale and zero codes (it reads back as
+// NaN and poisons only the queries that see it).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "b2m_internal.cuh"
+#include "ptx.cuh"
+#include "tc_common.cuh"
+
+namespace {
+
+using b2m::pdl_launch_dependents;
+using b2m::set_dev_error;
+
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_max_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Nearest e4m3 code (ties to even) of t, |t| <= 448. The hardware conversion
+// takes fp32, and rounding a double to fp32 first could land on a border that
+// the double is not on: t goes to fp32 toward zero with the lost bits ORed
+// into the last place, which the second rounding then sees as "above".
+__device__ __forceinline__ uint8_t e4m3_code(double t) {
+  float f = __double2float_rz(t);
+  if ((double)f != t) f = __uint_as_float(__float_as_uint(f) | 1u);
+  return (uint8_t)__nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3);
+}
+
+// The value a code stands for, before its row's scale.
+template <bool E4M3>
+__device__ __forceinline__ float code_value(uint8_t c) {
+  if (E4M3) return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+  return (float)(int8_t)c;
+}
+
+// One new row: quantised into codes[0..D) and *scale by one warp. `xs` is the
+// row's fp32 input staged in shared memory. norm: multiply by gain[d] /
+// sqrt(mean + eps) first; cos != null: rotary at `pos` on the first rot values.
+__device__ __forceinline__ void quantise_row(const float *xs, int D, const float *gain, double eps, const float *cos,
+                                             const float *sin, int64_t pos, int half, int rot, int interleaved,
+                                             bool e4m3, uint8_t *codes, float *scale, int lane) {
+  double inv = 1.0;
+  if (gain) {
+    double ss = 0.0;
+    for (int d = lane; d < D; d += 32) ss += (double)xs[d] * xs[d];
+    inv = 1.0 / sqrt(warp_sum_d(ss) / D + eps);
+  }
+  auto normed = [&](int d) { return gain ? (double)xs[d] * inv * gain[d] : (double)xs[d]; };
+  double x[8];  // D <= 256: four consecutive values of up to two 128-value blocks
+  double amax = 0.0;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int d = (i >> 2) * 128 + 4 * lane + (i & 3);
+    x[i] = 0.0;
+    if (d >= D) continue;
+    double v = normed(d);
+    if (cos && d < rot) {
+      const int hr = rot >> 1;
+      const bool first = interleaved ? (d & 1) == 0 : d < hr;
+      const int pi = interleaved ? d >> 1 : (first ? d : d - hr);
+      const int e = interleaved ? (d ^ 1) : (first ? d + hr : d - hr);
+      const double c = cos[pos * half + pi], sn = sin[pos * half + pi], w = normed(e);
+      v = first ? v * c - w * sn : v * c + w * sn;
+    }
+    x[i] = v;
+    bad |= !isfinite(v);
+    amax = fmax(amax, fabs(v));
+  }
+  bad = __any_sync(0xffffffffu, bad);
+  amax = warp_max_d(amax);
+  const double top = e4m3 ? 448.0 : 127.0;
+  const float s = bad ? __int_as_float(0x7fc00000) : (float)(amax / top);
+  if (lane == 0) *scale = s;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int d0 = h * 128 + 4 * lane;
+    if (d0 >= D) continue;
+    uint32_t w = 0;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      uint32_t c = 0;
+      if (s > 0.f) {  // false for NaN
+        const double t = fmin(fmax(x[4 * h + u] / (double)s, -top), top);
+        c = e4m3 ? e4m3_code(t) : (uint8_t)(int8_t)(int)rint(t);
+      }
+      w |= c << (8 * u);
+    }
+    if (d0 + 4 <= D && (reinterpret_cast<uintptr_t>(codes + d0) & 3) == 0) {
+      *reinterpret_cast<uint32_t *>(codes + d0) = w;
+    } else {
+      for (int u = 0; u < 4 && d0 + u < D; u++) codes[d0 + u] = (uint8_t)(w >> (8 * u));
+    }
+  }
+}
+
+// Rotary position of new token i of sequence b; -1 when its depth is outside
+// [0, S) (the caller raises the device error).
+__device__ __forceinline__ int64_t token_pos(const Kv8Args &a, int b, int i, int past) {
+  if (!a.depth) return past + i;
+  const int dp = a.depth[(int64_t)b * a.S + i];
+  return dp < 0 || dp >= a.S ? -1 : past + dp;
+}
+
+// Appends the call's keys and values, one warp per (token, kv head) and side.
+__global__ void __launch_bounds__(256) kv8_append_kernel(const Kv8Args a) {
+  pdl_launch_dependents();
+  __shared__ float stage[8][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 8 + warp;
+  if (item >= (int64_t)a.B * a.S * a.KVH * 2) return;
+  const int side = (int)(item & 1);
+  const int kvh = (int)((item >> 1) % a.KVH);
+  const int64_t bs = (item >> 1) / a.KVH;
+  const int i = (int)(bs % a.S), b = (int)(bs / a.S);
+  const int past = a.past[b];
+  const int64_t pos = token_pos(a, b, i, past);
+  if (past < 0 || (a.cos && pos < 0)) {
+    if (lane == 0 && a.err) set_dev_error(a.err, B2M_DEVERR_INDEX);
+    return;
+  }
+  if ((int64_t)past + i >= a.CAP) {
+    if (lane == 0 && a.err) set_dev_error(a.err, B2M_DEVERR_CACHE_FULL);
+    return;
+  }
+  const float *src = (side ? a.v : a.k) + ((int64_t)b * a.S + i) * a.kv_rs + (int64_t)kvh * a.D;
+  float *xs = stage[warp];
+  for (int d = lane; d < a.D; d += 32) xs[d] = src[d];
+  __syncwarp();
+  const int64_t row = ((int64_t)b * a.KVH + kvh) * a.CAP + past + i;
+  // rotary only reads the table where the position is in it: past + depth < CAP
+  const float *gain = side || !a.k_gain ? nullptr : a.k_gain + (int64_t)kvh * a.D;
+  const float *cos = side || pos >= a.CAP ? nullptr : a.cos;
+  quantise_row(xs, a.D, gain, a.eps, cos, a.sin, pos, a.half, a.rot, a.interleaved, a.e4m3,
+               (side ? a.vc : a.kc) + row * a.D, (side ? a.vs : a.ks) + row, lane);
+}
+
+// The values of n cached positions from start[b] (or 0) on, [B][KVH][n][D]
+// fp32: one warp per row.
+template <bool E4M3>
+__global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Args a, const int32_t *start, int n, float *k_out,
+                                                       float *v_out) {
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 8 + warp;
+  if (item >= (int64_t)a.B * a.KVH * n) return;
+  const int j = (int)(item % n);
+  const int64_t bk = item / n;
+  const int64_t pos = (int64_t)(start ? start[bk / a.KVH] : 0) + j;
+  if (pos < 0 || pos >= a.CAP) {
+    if (lane == 0 && a.err) set_dev_error(a.err, B2M_DEVERR_INDEX);
+    return;
+  }
+  const int64_t row = bk * a.CAP + pos;
+#pragma unroll
+  for (int side = 0; side < 2; side++) {
+    float *out = side ? v_out : k_out;
+    if (!out) continue;
+    const uint8_t *codes = (side ? a.vc : a.kc) + row * a.D;
+    const float s = (side ? a.vs : a.ks)[row];
+    for (int d = lane; d < a.D; d += 32) out[item * a.D + d] = code_value<E4M3>(codes[d]) * s;
+  }
+}
+
+// Moves rows past + path[j] to past + j for j < count, one warp per (layer,
+// sequence, kv head) and side. The path is strictly increasing with path[j] >=
+// j, so row j is read before any later step writes it. A path that is not
+// (or a count outside [0, n]) moves nothing and raises the device error.
+__global__ void __launch_bounds__(256) kv8_keep_kernel(const Kv8Args a, int layers, const int32_t *path,
+                                                       const int32_t *count, int n) {
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 8 + warp;
+  if (item >= (int64_t)layers * a.B * a.KVH * 2) return;
+  const int side = (int)(item & 1);
+  const int64_t lbk = item >> 1;  // (layer * B + b) * KVH + kvh
+  const int b = (int)((lbk / a.KVH) % a.B);
+  const int past = a.past[b], c = count[b];
+  const int32_t *p = path + (int64_t)b * n;
+  bool bad = past < 0 || c < 0 || c > n || (c > 0 && (int64_t)past + p[c - 1] >= a.CAP);
+  if (!bad)
+    for (int j = lane; j < c; j += 32) bad |= p[j] < j || p[j] >= n || (j > 0 && p[j] <= p[j - 1]);
+  if (__any_sync(0xffffffffu, bad)) {
+    if (lane == 0 && a.err) set_dev_error(a.err, B2M_DEVERR_INDEX);
+    return;
+  }
+  uint8_t *codes = side ? a.vc : a.kc;
+  float *scale = side ? a.vs : a.ks;
+  const int64_t base = lbk * a.CAP + past;
+  for (int j = 0; j < c; j++) {
+    const int64_t from = base + p[j], to = base + j;
+    if (from == to) continue;
+    for (int d = lane; d < a.D; d += 32) codes[to * a.D + d] = codes[from * a.D + d];
+    if (lane == 0) scale[to] = scale[from];
+    __syncwarp();
+  }
+}
+
+// Whether new token i of sequence b sees key j (past = cached positions).
+__device__ __forceinline__ bool sees(const Kv8Args &a, int j, int past, int i, uint64_t bits) {
+  if (!a.tree) return j <= past + i;
+  return j < past || (j - past < 64 && (bits >> (j - past) & 1));
+}
+
+// Attention in fp32 on the CUDA cores, any head_dim <= 256: CTA per (token,
+// query head, sequence), its eight warps taking keys in turn with an online
+// softmax each, merged in shared memory in warp order.
+template <bool E4M3>
+__global__ void __launch_bounds__(256) kv8_attend_kernel(const Kv8Args a) {
+  pdl_launch_dependents();
+  __shared__ float qs[256], wo[8][256], wm[8], wl[8];
+  __shared__ float sums[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int kvh = h / (a.H / a.KVH), D = a.D;
+  const int past = max(0, a.past[b]);
+  const int64_t pos = token_pos(a, b, i, past);
+  float x = tid < D ? a.q[((int64_t)b * a.S + i) * a.q_rs + (int64_t)h * D + tid] : 0.f;
+  if (a.q_gain) {
+    float ss = x * x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (lane == 0) sums[warp] = ss;
+    __syncthreads();
+    double t = 0.0;
+    for (int w = 0; w < 8; w++) t += sums[w];
+    const float inv = (float)(1.0 / sqrt(t / D + a.eps));
+    if (tid < D) x = x * inv * a.q_gain[(int64_t)h * D + tid];
+  }
+  qs[tid] = x;
+  __syncthreads();
+  if (a.cos && pos >= 0 && pos < a.CAP && tid < a.rot) {
+    const int hr = a.rot >> 1;
+    const bool first = a.interleaved ? (tid & 1) == 0 : tid < hr;
+    const int pi = a.interleaved ? tid >> 1 : (first ? tid : tid - hr);
+    const int e = a.interleaved ? (tid ^ 1) : (first ? tid + hr : tid - hr);
+    const float c = a.cos[pos * a.half + pi], sn = a.sin[pos * a.half + pi], w = qs[e];
+    x = first ? x * c - w * sn : x * c + w * sn;
+  }
+  __syncthreads();
+  qs[tid] = x * a.scale;
+  __syncthreads();
+  float q[8], o[8];
+#pragma unroll
+  for (int u = 0; u < 8; u++) {
+    q[u] = lane + 32 * u < D ? qs[lane + 32 * u] : 0.f;
+    o[u] = 0.f;
+  }
+  const uint64_t bits = a.tree ? a.tree[(int64_t)b * a.S + i] : 0;
+  const int kend = (int)min((int64_t)a.CAP, (int64_t)past + (a.tree ? a.S : i + 1));
+  const int64_t base = ((int64_t)b * a.KVH + kvh) * a.CAP;
+  float m = -INFINITY, l = 0.f;
+  for (int j = warp; j < kend; j += 8) {
+    if (!sees(a, j, past, i, bits)) continue;
+    const uint8_t *kr = a.kc + (base + j) * D, *vr = a.vc + (base + j) * D;
+    float t = 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (lane + 32 * u < D) t = fmaf(q[u], code_value<E4M3>(kr[lane + 32 * u]), t);
+#pragma unroll
+    for (int of = 16; of > 0; of >>= 1) t += __shfl_xor_sync(0xffffffffu, t, of);
+    t *= a.ks[base + j];
+    const float mn = fmaxf(m, t);
+    const float corr = m == -INFINITY ? 0.f : __expf(m - mn), p = __expf(t - mn);
+    const float pv = p * a.vs[base + j];
+    l = l * corr + p;
+    m = mn;
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (lane + 32 * u < D) o[u] = fmaf(pv, code_value<E4M3>(vr[lane + 32 * u]), o[u] * corr);
+  }
+  if (lane == 0) {
+    wm[warp] = m;
+    wl[warp] = l;
+  }
+#pragma unroll
+  for (int u = 0; u < 8; u++) wo[warp][lane + 32 * u] = o[u];
+  __syncthreads();
+  if (tid >= D) return;
+  float M = -INFINITY, L = 0.f, O = 0.f;
+  for (int w = 0; w < 8; w++) M = fmaxf(M, wm[w]);
+  for (int w = 0; w < 8; w++) {
+    // l == 0: this warp saw no key (its l is NaN, not 0, when a score was NaN)
+    const float f = wl[w] == 0.f ? 0.f : (wm[w] == -INFINITY ? 1.f : __expf(wm[w] - M));
+    L += wl[w] * f;
+    O += wo[w][tid] * f;
+  }
+  const float r = L == 0.f ? 0.f : O / L;  // a token that sees nothing: zeros
+  const int64_t at = ((int64_t)b * a.S + i) * a.H * D + (int64_t)h * D + tid;
+  if (a.out) a.out[at] = r;
+  if (a.out16) a.out16[at] = __float2half_rn(r);
+}
+
+unsigned blocks_for(int64_t items, int per) {
+  const int64_t g = (items + per - 1) / per;
+  B2M_REQUIRE(g <= 0x7fffffff, B2M_ERR_INVALID_ARGUMENT, "8-bit KV cache: too many rows in one call");
+  return (unsigned)g;
+}
+
+}  // namespace
+
+void launch_kv8_append(const Kv8Args &a, cudaStream_t s) {
+  const int64_t items = (int64_t)a.B * a.S * a.KVH * 2;
+  if (items == 0) return;
+  kv8_append_kernel<<<blocks_for(items, 8), 256, 0, s>>>(a);
+  B2M_CUDA(cudaGetLastError());
+}
+
+void launch_kv8_read(const Kv8Args &a, const int32_t *start, int n, float *k_out, float *v_out, cudaStream_t s) {
+  const int64_t items = (int64_t)a.B * a.KVH * n;
+  if (items == 0) return;
+  if (a.e4m3)
+    kv8_read_kernel<true><<<blocks_for(items, 8), 256, 0, s>>>(a, start, n, k_out, v_out);
+  else
+    kv8_read_kernel<false><<<blocks_for(items, 8), 256, 0, s>>>(a, start, n, k_out, v_out);
+  B2M_CUDA(cudaGetLastError());
+}
+
+void launch_kv8_keep(const Kv8Args &a, int layers, const int32_t *path, const int32_t *count, int n, cudaStream_t s) {
+  const int64_t items = (int64_t)layers * a.B * a.KVH * 2;
+  if (items == 0 || n == 0) return;
+  kv8_keep_kernel<<<blocks_for(items, 8), 256, 0, s>>>(a, layers, path, count, n);
+  B2M_CUDA(cudaGetLastError());
+}
+
+void launch_kv8_attend(const Kv8Args &a, bool exact, cudaStream_t s) {
+  (void)exact;
+  launch_kv8_append(a, s);
+  const dim3 grid((unsigned)a.S, (unsigned)a.H, (unsigned)a.B);
+  if (a.e4m3)
+    kv8_attend_kernel<true><<<grid, 256, 0, s>>>(a);
+  else
+    kv8_attend_kernel<false><<<grid, 256, 0, s>>>(a);
+  B2M_CUDA(cudaGetLastError());
+}

@@ -2073,6 +2073,165 @@ B2M_API b2m_status b2m_advance_positions_dev(b2m_ctx *ctx, int32_t *past, int32_
 }
 
 // ---------------------------------------------------------------------------
+// 8-bit KV cache and log probabilities. The arguments are checked before the
+// context, so that every refusal can be met without a device.
+// ---------------------------------------------------------------------------
+
+// The cache's own checks; `used`: the call touches at least one row.
+static Kv8Args kv8_cache_args(const b2m_kv8_cache *c, bool used, const char *what) {
+  const std::string w(what);
+  B2M_REQUIRE(c, B2M_ERR_INVALID_ARGUMENT, w + ": cache is null");
+  B2M_REQUIRE(c->type == B2M_INT8 || c->type == B2M_FLOAT8E4M3FN, B2M_ERR_UNSUPPORTED,
+              w + ": the cache type must be INT8 or FLOAT8E4M3FN");
+  B2M_REQUIRE(c->b >= 0 && c->kvh > 0 && c->cap > 0 && c->head_dim > 0 && c->head_dim <= 256,
+              B2M_ERR_INVALID_ARGUMENT, w + ": bad cache shape");
+  B2M_REQUIRE(!used || (c->k && c->v && c->k_scale && c->v_scale), B2M_ERR_INVALID_ARGUMENT,
+              w + ": null cache pointer");
+  auto al4 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; };
+  B2M_REQUIRE(al4(c->k) && al4(c->v) && al4(c->k_scale) && al4(c->v_scale), B2M_ERR_INVALID_ARGUMENT,
+              w + ": cache pointers must be 4-byte aligned");
+  Kv8Args a;
+  a.kc = static_cast<uint8_t *>(c->k);
+  a.vc = static_cast<uint8_t *>(c->v);
+  a.ks = c->k_scale;
+  a.vs = c->v_scale;
+  a.e4m3 = c->type == B2M_FLOAT8E4M3FN;
+  a.B = c->b, a.KVH = c->kvh, a.CAP = c->cap, a.D = c->head_dim;
+  return a;
+}
+
+static void kv8_rotary_args(Kv8Args &a, const float *cos_cache, const float *sin_cache, int32_t rotary_half,
+                            int32_t rotary_dim, int32_t interleaved, const char *what) {
+  B2M_REQUIRE(!cos_cache || (sin_cache && rotary_half > 0 && rotary_dim > 0 && rotary_dim <= a.D &&
+                             rotary_dim % 2 == 0 && rotary_dim / 2 <= rotary_half),
+              B2M_ERR_INVALID_ARGUMENT, std::string(what) + ": bad rotary arguments");
+  if (!cos_cache) return;
+  a.cos = cos_cache, a.sin = sin_cache;
+  a.half = rotary_half, a.rot = rotary_dim, a.interleaved = interleaved ? 1 : 0;
+}
+
+B2M_API b2m_status b2m_kv8_append_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const float *k, const float *v,
+                                      int64_t kv_rs, const float *k_gain, double eps, const int32_t *past,
+                                      const int32_t *depth, const float *cos_cache, const float *sin_cache,
+                                      int32_t rotary_half, int32_t rotary_dim, int32_t interleaved, int32_t s) {
+  return guarded([&] {
+    const char *what = "KV cache append";
+    const bool used = cache && s > 0 && cache->b > 0;
+    Kv8Args a = kv8_cache_args(cache, used, what);
+    B2M_REQUIRE(s >= 0 && (!used || (k && v && past)), B2M_ERR_INVALID_ARGUMENT,
+                "KV cache append: bad token count or null pointer");
+    B2M_REQUIRE(kv_rs >= (int64_t)a.KVH * a.D, B2M_ERR_INVALID_ARGUMENT, "KV cache append: row stride too small");
+    B2M_REQUIRE(!k_gain || eps >= 0.0, B2M_ERR_INVALID_ARGUMENT, "KV cache append: eps must be >= 0");
+    kv8_rotary_args(a, cos_cache, sin_cache, rotary_half, rotary_dim, interleaved, what);
+    check_ctx(ctx);
+    if (!used) return;
+    check_cancel(ctx);
+    a.err = ctx->dev_err;
+    a.k = k, a.v = v, a.kv_rs = kv_rs, a.k_gain = k_gain, a.eps = eps;
+    a.past = past, a.depth = depth, a.S = s;
+    DeviceGuard dg(ctx->device);
+    OpTimer tm(ctx);
+    launch_kv8_append(a, ctx->stream);
+    tm.done();
+  });
+}
+
+B2M_API b2m_status b2m_kv8_read_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const int32_t *start, int32_t n,
+                                    float *k_out, float *v_out) {
+  return guarded([&] {
+    const bool used = cache && n > 0 && cache->b > 0 && (k_out || v_out);
+    Kv8Args a = kv8_cache_args(cache, used, "KV cache read");
+    B2M_REQUIRE(n >= 0 && n <= a.CAP, B2M_ERR_INVALID_ARGUMENT, "KV cache read: n must lie in [0, cap]");
+    check_ctx(ctx);
+    if (!used) return;
+    check_cancel(ctx);
+    a.err = ctx->dev_err;
+    DeviceGuard dg(ctx->device);
+    OpTimer tm(ctx);
+    launch_kv8_read(a, start, n, k_out, v_out, ctx->stream);
+    tm.done();
+  });
+}
+
+B2M_API b2m_status b2m_gqa_kv8_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const float *q, const float *k,
+                                   const float *v, int64_t q_rs, int64_t kv_rs, const float *qk_gain, double eps,
+                                   const int32_t *past, const uint64_t *tree, const int32_t *depth,
+                                   const float *cos_cache, const float *sin_cache, int32_t rotary_half,
+                                   int32_t rotary_dim, int32_t interleaved, float *out, uint16_t *out16, int32_t s,
+                                   int32_t h, float scale) {
+  return guarded([&] {
+    const char *what = "GroupQueryAttention (8-bit cache)";
+    const std::string w(what);
+    const bool used = cache && s > 0 && cache->b > 0;
+    Kv8Args a = kv8_cache_args(cache, used, what);
+    B2M_REQUIRE(s >= 0 && h > 0 && h % a.KVH == 0 && h <= 65535 && a.B <= 65535, B2M_ERR_INVALID_ARGUMENT,
+                w + ": bad shape arguments");
+    B2M_REQUIRE(!used || (q && k && v && past && (out || out16)), B2M_ERR_INVALID_ARGUMENT, w + ": null pointer");
+    B2M_REQUIRE(q_rs >= (int64_t)h * a.D && kv_rs >= (int64_t)a.KVH * a.D, B2M_ERR_INVALID_ARGUMENT,
+                w + ": row strides too small");
+    B2M_REQUIRE(!tree == !depth, B2M_ERR_INVALID_ARGUMENT, w + ": tree and depth go together");
+    B2M_REQUIRE(!tree || s <= 64, B2M_ERR_UNSUPPORTED, w + ": a drafted tree has at most 64 tokens");
+    B2M_REQUIRE(!qk_gain || eps >= 0.0, B2M_ERR_INVALID_ARGUMENT, w + ": eps must be >= 0");
+    B2M_REQUIRE(!out16 || (int64_t)h * a.D % 8 == 0, B2M_ERR_INVALID_ARGUMENT,
+                w + ": h * head_dim must be a multiple of 8 for the f16 output");
+    kv8_rotary_args(a, cos_cache, sin_cache, rotary_half, rotary_dim, interleaved, what);
+    check_ctx(ctx);
+    if (!used) return;
+    check_cancel(ctx);
+    a.err = ctx->dev_err;
+    a.S = s, a.H = h;
+    a.q = q, a.k = k, a.v = v, a.q_rs = q_rs, a.kv_rs = kv_rs;
+    a.q_gain = qk_gain, a.k_gain = qk_gain ? qk_gain + (int64_t)h * a.D : nullptr, a.eps = eps;
+    a.past = past, a.tree = tree, a.depth = depth;
+    a.scale = scale > 0.f ? scale : 1.f / std::sqrt((float)a.D);
+    a.out = out, a.out16 = reinterpret_cast<__half *>(out16);
+    DeviceGuard dg(ctx->device);
+    OpTimer tm(ctx);
+    launch_kv8_attend(a, ctx->attn_exact, ctx->stream);
+    tm.done();
+  });
+}
+
+B2M_API b2m_status b2m_kv8_keep_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, int32_t layers, const int32_t *past,
+                                    const int32_t *path, const int32_t *count, int32_t n) {
+  return guarded([&] {
+    const bool used = cache && cache->b > 0 && layers > 0 && n > 0;
+    Kv8Args a = kv8_cache_args(cache, used, "KV cache keep");
+    B2M_REQUIRE(layers >= 0 && n >= 0, B2M_ERR_INVALID_ARGUMENT, "KV cache keep: negative layers or n");
+    B2M_REQUIRE(!used || (past && path && count), B2M_ERR_INVALID_ARGUMENT, "KV cache keep: null pointer");
+    check_ctx(ctx);
+    if (!used) return;
+    check_cancel(ctx);
+    a.err = ctx->dev_err;
+    a.past = past;
+    DeviceGuard dg(ctx->device);
+    OpTimer tm(ctx);
+    launch_kv8_keep(a, layers, path, count, n, ctx->stream);
+    tm.done();
+  });
+}
+
+B2M_API b2m_status b2m_logprobs_dev(b2m_ctx *ctx, const float *logits, int64_t ld, const int64_t *ids, int64_t rows,
+                                    int64_t v, float *logprob, float *entropy, int32_t k, int64_t *top_ids,
+                                    float *top_logprobs) {
+  return guarded([&] {
+    B2M_REQUIRE(rows >= 0 && v > 0 && v < ((int64_t)1 << 31) && ld >= v && (rows == 0 || logits),
+                B2M_ERR_INVALID_ARGUMENT, "LogProbs: bad arguments");
+    B2M_REQUIRE(!ids == !logprob, B2M_ERR_INVALID_ARGUMENT, "LogProbs: ids and logprob go together");
+    B2M_REQUIRE(k >= 0 && k <= B2M_LOGPROBS_MAX_K && k <= v, B2M_ERR_INVALID_ARGUMENT,
+                "LogProbs: k must lie in [0, min(32, v)]");
+    B2M_REQUIRE(rows == 0 || k == 0 || top_ids, B2M_ERR_INVALID_ARGUMENT, "LogProbs: top_ids is null");
+    check_ctx(ctx);
+    if (rows == 0) return;
+    check_cancel(ctx);
+    DeviceGuard dg(ctx->device);
+    OpTimer tm(ctx);
+    launch_logprobs(logits, ld, ids, rows, v, logprob, entropy, k, top_ids, top_logprobs, ctx->dev_err, ctx->stream);
+    tm.done();
+  });
+}
+
+// ---------------------------------------------------------------------------
 // Conv / ConvInteger / QLinearConv: im2col panels on the device feeding the
 // fp32 and int8 GEMM kernels (opConv, lib/src/onnx_nn_ops.dart:179-545;
 // opConvInteger / opQLinearConv, lib/src/onnx_qlinear_ops.dart:230-382).

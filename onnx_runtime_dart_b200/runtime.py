@@ -261,6 +261,16 @@ class PackedWeight:
             pass
 
 
+def use_torch_stream(ctx: Context) -> None:
+    """Enqueues the context's later calls on torch's current stream of its
+    device, the legacy default stream included (torch names it 0, which
+    b2m_set_stream takes for the context's own; CUDA's explicit handle of it,
+    cudaStreamLegacy, is 1). Call it again after changing torch's stream."""
+    import torch
+
+    ctx.set_stream(torch.cuda.current_stream(ctx.device).cuda_stream or 1)
+
+
 @contextlib.contextmanager
 def torch_stream_scope(ctx: Context, torch, own):
     """Orders the enclosed library calls with torch's current stream.
