@@ -1,0 +1,558 @@
+// Attention over the 8-bit KV cache for few query rows per kv head: a decode
+// step (the G query heads of a group), a small drafted tree or a short chunk.
+//
+// A cluster of CL CTAs serves one (kv head, sequence, tile of 8 NT query rows);
+// its CTAs take consecutive key ranges, the four warps of a CTA 16-key tiles of
+// its range in turn. Per tile a warp forms, with mma.m16n8k16 (f16 operands,
+// fp32 sums),
+//   S^T[16 keys][8 rows] = K . Q^T,   O^T[D][8 rows] += V^T . P^T.
+// The codes are the A operands: int8 and e4m3 codes are f16 numbers exactly, so
+// they are expanded in registers and the scales applied in fp32, K's to the
+// scores and V's to the weights. Q and the weights are split into two f16 terms
+// (22 bits), so the products carry fp32 accuracy. Which D index or key an MMA
+// lane holds is free as long as both operands agree: lanes are given 16
+// consecutive bytes of a row, so no data is shuffled on its way to the tensor
+// cores; only P^T is transposed between the two products (movmatrix).
+//
+// Bound by HBM (2 D + 8 bytes per key of a kv head). Each lane copies the bytes
+// it will use itself into a ring of its own in shared memory (cp.async), three
+// tiles ahead, so that enough loads are in flight without registers and no
+// barrier is needed in the loop.
+//
+// The softmax reference m moves only when a score passes it by more than 2^5 (a
+// warp vote); weights are scaled by 2^10 so that f16 keeps small ones. V scales
+// are taken relative to the largest seen (2^ev). Warps, then the cluster's CTAs,
+// merge in a fixed order through (distributed) shared memory: no workspace and
+// no atomics, so captured graphs share nothing and results repeat.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "kv8_common.cuh"
+#include "tc_common.cuh"
+
+namespace {
+
+namespace cg = cooperative_groups;
+using namespace kv8;
+
+constexpr int ST_WARPS = 4, ST_THREADS = 32 * ST_WARPS, ST_STAGES = 4;
+constexpr float P_BIAS = 10.f, M_SLACK = 5.f;  // log2: weights below 2^15 fit f16
+
+template <int N>
+__device__ __forceinline__ void cp_async(void *dst, const void *src) {
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(b2m::smem_u32(dst)), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(b2m::smem_u32(dst)), "l"(src), "n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// How a row of D codes is dealt to the lanes: K rows in NKC chunks of KC bytes
+// for each of four lanes, V rows in NVC chunks of VC bytes for each of eight.
+template <int D>
+struct StepShape {
+  static_assert(D % 32 == 0 && D <= 256, "head dim");
+  static constexpr int KC = D % 64 == 0 ? 16 : 8, NKC = D / (4 * KC), KW = KC / 4;
+  static constexpr int VC = D % 128 == 0 ? 16 : (D % 64 == 0 ? 8 : 4), NVC = D / (8 * VC), VW = VC / 4;
+  static constexpr int KSTEPS = D / 16, MT = D / 16;
+  // One ring slot of a warp: K chunks [row half][chunk][lane], V chunks
+  // [key slot][chunk][lane], one scale per lane.
+  static constexpr int K_BYTES = 2 * NKC * 32 * KC, V_BYTES = 4 * NVC * 32 * VC, SLOT = K_BYTES + V_BYTES + 128;
+};
+
+template <int D, int NT>
+struct StepSmem {
+  static constexpr int R = 8 * NT;
+  static constexpr int RING = 0;
+  static constexpr int QF = RING + ST_WARPS * ST_STAGES * StepShape<D>::SLOT;  // Q fragments [NT][KSTEPS][32] uint4
+  static constexpr int ROWS = QF + NT * StepShape<D>::KSTEPS * 512;            // per-row words, below
+  // bits[R] (u64), factor[R], lim[R], wm[4][R], wl[4][R], cm[R], cl[R]
+  static constexpr int BYTES = ROWS + R * (8 + 4 + 4 + 16 + 16 + 8);
+  // Warp states O [4][R][D] fp32, and the prologue's staging rows, reuse the
+  // ring (drained by then / not yet filled).
+  static_assert(ST_WARPS * R * D * 4 <= QF, "O staging fits the ring");
+  static_assert((R + ST_WARPS) * 256 * 4 <= QF || (R * D + ST_WARPS * 256) * 4 <= QF, "Q staging fits the ring");
+};
+
+template <bool E4M3, int D, int NT>
+__global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, const int fused_append) {
+  using L = StepShape<D>;
+  using M = StepSmem<D, NT>;
+  constexpr int R = M::R;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint8_t *rows_mem = smem + M::ROWS;
+  uint64_t *row_bits = reinterpret_cast<uint64_t *>(rows_mem);
+  float *row_factor = reinterpret_cast<float *>(rows_mem + 8 * R);
+  int *row_lim = reinterpret_cast<int *>(rows_mem + 12 * R);
+  float *wm = reinterpret_cast<float *>(rows_mem + 16 * R), *wl = wm + ST_WARPS * R, *cm = wl + ST_WARPS * R,
+        *cl_ = cm + R;
+  uint4 *qfrag = reinterpret_cast<uint4 *>(smem + M::QF);
+
+  b2m::pdl_launch_dependents();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int g = lane >> 2, t = lane & 3;
+  const int row0 = (int)(blockIdx.x / CL) * R, kvh = blockIdx.y, b = blockIdx.z;
+  const int G = a.H / a.KVH, nrows = a.S * G;
+  const int past = max(0, a.past[b]);
+  // keys that the tile's last row sees
+  const int n = (int)min((int64_t)a.CAP, (int64_t)past + (a.tree ? a.S : min(a.S, (row0 + R - 1) / G + 1)));
+  const int chunk = (((n + CL - 1) / CL) + 15) & ~15;
+  const int jbeg = min(n, rank * chunk), jend = min(n, jbeg + chunk);
+  const int64_t base = ((int64_t)b * a.KVH + kvh) * a.CAP;
+
+  // New rows that fall into this CTA's range (every rank sees to its own, the
+  // last one also reports those past the capacity).
+  if (fused_append) {
+    float *stage = reinterpret_cast<float *>(smem) + warp * 256;
+    const int i0 = max(0, jbeg - past), i1 = rank == CL - 1 ? a.S : min(a.S, jend - past);
+    for (int it = 2 * i0 + warp; it < 2 * i1; it += ST_WARPS)
+      if (past + (it >> 1) >= jbeg) append_row(a, b, it >> 1, kvh, it & 1, a.past[b], stage, lane);
+    __syncthreads();
+  }
+
+  // Q rows: head norm, rotary, scaled to a largest magnitude in [2^9, 2^10) by a
+  // power of two that joins the row's factor.
+  {
+    float *qs = reinterpret_cast<float *>(smem) + ST_WARPS * 256;
+    for (int rr = warp; rr < R; rr += ST_WARPS) {
+      const int r = row0 + rr;
+      float *x = qs + rr * D;
+      const bool valid = r < nrows;
+      const int i = valid ? r / G : 0, h = kvh * G + (valid ? r % G : 0);
+      const float *src = a.q + ((int64_t)b * a.S + i) * a.q_rs + (int64_t)h * D;
+      float v[D / 32];
+      float ss = 0.f;
+#pragma unroll
+      for (int u = 0; u < D / 32; u++) {
+        v[u] = valid ? src[lane + 32 * u] : 0.f;
+        ss = fmaf(v[u], v[u], ss);
+      }
+      if (a.q_gain) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = (float)(1.0 / sqrt((double)ss / D + a.eps));
+#pragma unroll
+        for (int u = 0; u < D / 32; u++) v[u] = valid ? v[u] * inv * a.q_gain[(int64_t)h * D + lane + 32 * u] : 0.f;
+      }
+      if (a.cos) {
+#pragma unroll
+        for (int u = 0; u < D / 32; u++) x[lane + 32 * u] = v[u];
+        __syncwarp();
+        const int64_t pos = token_pos(a, b, i, past);
+        if (valid && pos >= 0 && pos < a.CAP) {
+          const int hr = a.rot >> 1;
+#pragma unroll
+          for (int u = 0; u < D / 32; u++) {
+            const int d = lane + 32 * u;
+            if (d >= a.rot) continue;
+            const bool first = a.interleaved ? (d & 1) == 0 : d < hr;
+            const int pi = a.interleaved ? d >> 1 : (first ? d : d - hr);
+            const int e = a.interleaved ? (d ^ 1) : (first ? d + hr : d - hr);
+            const float c = a.cos[pos * a.half + pi], sn = a.sin[pos * a.half + pi], w = x[e];
+            v[u] = first ? v[u] * c - w * sn : v[u] * c + w * sn;
+          }
+        }
+        __syncwarp();
+      }
+      float mx = 0.f;
+#pragma unroll
+      for (int u = 0; u < D / 32; u++) mx = fmaxf(mx, fabsf(v[u]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      // mx = f 2^e with f in [1/2, 1): scaled by 2^(10 - e). Zero, infinite and
+      // (ignored by fmaxf) NaN rows: any exponent does.
+      int e = 10;
+      if (mx > 0.f && mx < INFINITY) frexpf(mx, &e);
+#pragma unroll
+      for (int u = 0; u < D / 32; u++) x[lane + 32 * u] = ldexpf(v[u], 10 - e);
+      if (lane == 0) {
+        row_factor[rr] = ldexpf(a.scale * LOG2E * code_factor<E4M3>(), e - 10);
+        row_lim[rr] = !valid ? -1 : (a.tree ? past - 1 : past + i);
+        row_bits[rr] = valid && a.tree ? a.tree[(int64_t)b * a.S + i] : 0;
+      }
+    }
+    __syncthreads();
+    // Fragments: element pairs of a k-step in the order the codes' words give.
+    for (int e = tid; e < NT * L::KSTEPS * 32; e += ST_THREADS) {
+      const int ln = e & 31, ks = (e >> 5) % L::KSTEPS, nt = (e >> 5) / L::KSTEPS;
+      const int d = ((ks / L::KW) * 4 + (ln & 3)) * L::KC + 4 * (ks % L::KW);
+      const float4 x = *reinterpret_cast<const float4 *>(qs + (nt * 8 + (ln >> 2)) * D + d);
+      const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
+      const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+      qfrag[e] = make_uint4(b2m::h2_as_u32(h0), b2m::h2_as_u32(h1),
+                            b2m::h2_as_u32(__floats2half2_rn(x.x - f0.x, x.y - f0.y)),
+                            b2m::h2_as_u32(__floats2half2_rn(x.z - f1.x, x.w - f1.y)));
+    }
+    __syncthreads();
+  }
+
+  // Ring of this warp.
+  uint8_t *ring = smem + warp * (ST_STAGES * L::SLOT);
+  const uint8_t *kcodes = a.kc + base * D, *vcodes = a.vc + base * D;
+  const float *kscale = a.ks + base, *vscale = a.vs + base;
+  const int ntile = (jend - jbeg + 15) >> 4;
+  auto issue = [&](int tile, int slot) {
+    if (tile < ntile) {
+      const int j0 = jbeg + 16 * tile;
+      uint8_t *s = ring + slot * L::SLOT;
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        const uint8_t *src = kcodes + (int64_t)min(j0 + 8 * hf + g, jend - 1) * D + t * L::KC;
+#pragma unroll
+        for (int c = 0; c < L::NKC; c++)
+          cp_async<L::KC>(s + ((hf * L::NKC + c) * 32 + lane) * L::KC, src + c * 4 * L::KC);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; q++) {  // keys 2t, 2t+1, 2t+8, 2t+9
+        const uint8_t *src = vcodes + (int64_t)min(j0 + 2 * t + (q & 1) + 8 * (q >> 1), jend - 1) * D + g * L::VC;
+#pragma unroll
+        for (int c = 0; c < L::NVC; c++)
+          cp_async<L::VC>(s + L::K_BYTES + ((q * L::NVC + c) * 32 + lane) * L::VC, src + c * 8 * L::VC);
+      }
+      // lane t of a group: K scale of keys g, g + 8, V scale of keys g, g + 8
+      const float *sp = (t & 2 ? vscale : kscale) + min(j0 + g + 8 * (t & 1), jend - 1);
+      cp_async<4>(s + L::K_BYTES + L::V_BYTES + lane * 4, sp);
+    }
+    cp_commit();
+  };
+
+  float o[NT][L::MT][4];
+  float m[NT][2], mref[NT][2], l[NT][2], rf[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+    for (int k = 0; k < L::MT; k++)
+#pragma unroll
+      for (int u = 0; u < 4; u++) o[nt][k][u] = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      m[nt][u] = -INFINITY;
+      mref[nt][u] = 0.f;
+      l[nt][u] = 0.f;
+      rf[nt][u] = row_factor[nt * 8 + 2 * t + u];
+    }
+  }
+  float vmax = 0.f, vinv = 0.f;  // largest V scale seen (a power of two above it), and its reciprocal
+  const int all_see = a.tree ? past : past + row0 / G + 1;  // keys below this are seen by every row
+
+#pragma unroll
+  for (int s = 0; s < ST_STAGES - 1; s++) issue(warp + s * ST_WARPS, s);
+  int slot = 0;
+  for (int tile = warp; tile < ntile; tile += ST_WARPS) {
+    cp_wait<ST_STAGES - 2>();
+    __syncwarp();
+    issue(tile + (ST_STAGES - 1) * ST_WARPS, slot == 0 ? ST_STAGES - 1 : slot - 1);
+    const uint8_t *s = ring + slot * L::SLOT;
+    const int j0 = jbeg + 16 * tile;
+    // S^T = K . Q^T
+    float c[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int u = 0; u < 4; u++) c[nt][u] = 0.f;
+#pragma unroll
+    for (int cc = 0; cc < L::NKC; cc++) {
+      uint32_t w0[L::KW], w1[L::KW];
+      const uint8_t *p0 = s + (cc * 32 + lane) * L::KC, *p1 = p0 + L::NKC * 32 * L::KC;
+      if constexpr (L::KC == 16) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(p0), y = *reinterpret_cast<const uint4 *>(p1);
+        w0[0] = x.x, w0[1] = x.y, w0[2] = x.z, w0[3] = x.w;
+        w1[0] = y.x, w1[1] = y.y, w1[2] = y.z, w1[3] = y.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2 *>(p0), y = *reinterpret_cast<const uint2 *>(p1);
+        w0[0] = x.x, w0[1] = x.y;
+        w1[0] = y.x, w1[1] = y.y;
+      }
+#pragma unroll
+      for (int w = 0; w < L::KW; w++) {
+        uint32_t A[4];
+        expand4<E4M3>(w0[w], A[0], A[2]);
+        expand4<E4M3>(w1[w], A[1], A[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          const uint4 q = qfrag[(nt * L::KSTEPS + cc * L::KW + w) * 32 + lane];
+          b2m::mma_16816(c[nt], A, q.x, q.y, c[nt]);
+          b2m::mma_16816(c[nt], A, q.z, q.w, c[nt]);
+        }
+      }
+    }
+    // Scores in log2 units; masked ones -inf.
+    const float4 sc = *reinterpret_cast<const float4 *>(s + L::K_BYTES + L::V_BYTES + g * 16);
+    float x[NT][2][2];  // [key g, g + 8][row 2t, 2t + 1]
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        x[nt][0][u] = c[nt][u] * sc.x * rf[nt][u];
+        x[nt][1][u] = c[nt][2 + u] * sc.y * rf[nt][u];
+      }
+    const bool whole = j0 + 16 <= min(jend, all_see);
+    uint32_t seen = 0xffffffffu;  // bit (nt * 2 + key) * 2 + row
+    if (!whole) {
+      seen = 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            const int j = j0 + g + 8 * k, rr = nt * 8 + 2 * t + u, dj = j - past;
+            const bool ok = j < jend && (j <= row_lim[rr] || (dj >= 0 && dj < 64 && (row_bits[rr] >> dj & 1)));
+            if (ok)
+              seen |= 1u << ((nt * 2 + k) * 2 + u);
+            else
+              x[nt][k][u] = -INFINITY;
+          }
+    }
+    // Keys past the range stand for its last key: their scales are valid ones.
+    bool need = fmaxf(sc.z, sc.w) > vmax;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) need |= fmaxf(x[nt][0][u], x[nt][1][u]) > m[nt][u] + M_SLACK;
+    if (__any_sync(0xffffffffu, need)) {
+      float vm = fmaxf(sc.z, sc.w);
+#pragma unroll
+      for (int of = 4; of < 32; of <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, of));
+      float vf = 1.f;  // old reference over new one
+      if (vm > vmax) {
+        // the power of two above vm, kept where its reciprocal is a normal number
+        const float up = __uint_as_float(min(max((__float_as_uint(vm) >> 23) + 1u, 2u), 252u) << 23);
+        vf = vmax * (1.f / up);
+        vmax = up;
+        vinv = 1.f / up;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          float tm = fmaxf(x[nt][0][u], x[nt][1][u]);
+#pragma unroll
+          for (int of = 4; of < 32; of <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, of));
+          const float mn = fmaxf(m[nt][u], tm);
+          const float f = m[nt][u] == -INFINITY ? 0.f : ex2(m[nt][u] - mn);
+          if (mn > m[nt][u]) {
+            l[nt][u] = l[nt][u] == 0.f ? 0.f : l[nt][u] * f;
+            m[nt][u] = mn;
+            mref[nt][u] = mn - P_BIAS;
+          }
+          const float fo = (mn == -INFINITY ? 1.f : f) * vf;
+#pragma unroll
+          for (int k = 0; k < L::MT; k++) {
+            o[nt][k][u] *= fo;
+            o[nt][k][2 + u] *= fo;
+          }
+        }
+    }
+    // Weights (with V's scales) as two f16 terms, transposed into B fragments.
+    const float v0 = sc.z * vinv, v1 = sc.w * vinv;
+    uint32_t bh[NT][2], bl[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        float w[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const bool ok = seen >> ((nt * 2 + k) * 2 + u) & 1;
+          const float p = ok ? ex2(x[nt][k][u] - mref[nt][u]) : 0.f;
+          l[nt][u] += p;
+          w[u] = ok ? p * (k ? v1 : v0) : 0.f;  // a hidden key's scale may be NaN
+        }
+        const __half2 h = __floats2half2_rn(w[0], w[1]);
+        const float2 hf = __half22float2(h);
+        bh[nt][k] = transpose8x8(b2m::h2_as_u32(h));
+        bl[nt][k] = transpose8x8(b2m::h2_as_u32(__floats2half2_rn(w[0] - hf.x, w[1] - hf.y)));
+      }
+    // O^T += V^T . P^T
+#pragma unroll
+    for (int cc = 0; cc < L::NVC; cc++) {
+      uint32_t vw[4][L::VW];
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const uint8_t *p = s + L::K_BYTES + ((q * L::NVC + cc) * 32 + lane) * L::VC;
+        if constexpr (L::VC == 16) {
+          const uint4 y = *reinterpret_cast<const uint4 *>(p);
+          vw[q][0] = y.x, vw[q][1] = y.y, vw[q][2] = y.z, vw[q][3] = y.w;
+        } else if constexpr (L::VC == 8) {
+          const uint2 y = *reinterpret_cast<const uint2 *>(p);
+          vw[q][0] = y.x, vw[q][1] = y.y;
+        } else {
+          vw[q][0] = *reinterpret_cast<const uint32_t *>(p);
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < L::VW; w++) {
+        uint32_t A[2][4];  // dims 4w, 4w+1 and 4w+2, 4w+3 of the chunk
+        expand4<E4M3>(b2m::prmt(vw[0][w], vw[1][w], PAIR01), A[0][0], A[0][1]);
+        expand4<E4M3>(b2m::prmt(vw[2][w], vw[3][w], PAIR01), A[0][2], A[0][3]);
+        expand4<E4M3>(b2m::prmt(vw[0][w], vw[1][w], PAIR23), A[1][0], A[1][1]);
+        expand4<E4M3>(b2m::prmt(vw[2][w], vw[3][w], PAIR23), A[1][2], A[1][3]);
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            float *acc = o[nt][(cc * L::VW + w) * 2 + hf];
+            b2m::mma_16816(acc, A[hf], bh[nt][0], bh[nt][1], acc);
+            b2m::mma_16816(acc, A[hf], bl[nt][0], bl[nt][1], acc);
+          }
+      }
+    }
+    slot = slot + 1 == ST_STAGES ? 0 : slot + 1;
+    __syncwarp();  // every lane has read the slot's scales before it is refilled
+  }
+  cp_wait<0>();
+  __syncthreads();  // the rings are drained: the states reuse them
+
+  // Warp states: m, l per row and O (in the values' own scale).
+  float *so = reinterpret_cast<float *>(smem);
+  const float vs_out = vmax * code_factor<E4M3>();
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      float s = l[nt][u];
+#pragma unroll
+      for (int of = 4; of < 32; of <<= 1) s += __shfl_xor_sync(0xffffffffu, s, of);
+      const int rr = nt * 8 + 2 * t + u;
+      if (g == 0) {
+        wm[warp * R + rr] = m[nt][u];
+        wl[warp * R + rr] = s;
+      }
+      float *dst = so + (warp * R + rr) * D;
+#pragma unroll
+      for (int k = 0; k < L::MT; k++) {
+        const int cc = (k >> 1) / L::VW, w = (k >> 1) % L::VW;
+        const int d = (cc * 8 + g) * L::VC + 4 * w + 2 * (k & 1);
+        *reinterpret_cast<float2 *>(dst + d) = make_float2(o[nt][k][u] * vs_out, o[nt][k][2 + u] * vs_out);
+      }
+    }
+  __syncthreads();
+  // A state's share of the joint one: none if it saw no key; with a NaN sum and
+  // no maximum (all its scores NaN) it passes the NaN on.
+  auto share = [](float sm, float sl, float top) {
+    return sl == 0.f ? 0.f : (sm == -INFINITY ? 1.f : ex2(sm - top));
+  };
+  constexpr int D4 = D / 4;
+  for (int e = tid; e < R * D4; e += ST_THREADS) {
+    const int rr = e / D4;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < ST_WARPS; w++) top = fmaxf(top, wm[w * R + rr]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < ST_WARPS; w++) {
+      const float sl = wl[w * R + rr], f = share(wm[w * R + rr], sl, top);
+      const float4 v = reinterpret_cast<const float4 *>(so + w * R * D)[e];
+      sum += sl * f;
+      acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+    }
+    reinterpret_cast<float4 *>(so)[e] = acc;
+    if (e % D4 == 0) {
+      cm[rr] = top;
+      cl_[rr] = sum;
+    }
+  }
+  if (CL > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  for (int e = rank * ST_THREADS + tid; e < R * D4; e += CL * ST_THREADS) {
+    const int rr = e / D4, r = row0 + rr;
+    if (r >= nrows) continue;
+    float top = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < CL; q++) top = fmaxf(top, CL > 1 ? *cluster.map_shared_rank(cm + rr, q) : cm[rr]);
+    for (int q = 0; q < CL; q++) {
+      const float sl = CL > 1 ? *cluster.map_shared_rank(cl_ + rr, q) : cl_[rr];
+      const float sm = CL > 1 ? *cluster.map_shared_rank(cm + rr, q) : cm[rr];
+      const float f = share(sm, sl, top);
+      const float4 *src = reinterpret_cast<const float4 *>(so) + e;
+      const float4 v = CL > 1 ? *cluster.map_shared_rank(src, q) : *src;
+      sum += sl * f;
+      acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that saw nothing: zeros
+    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+    const int64_t at = ((int64_t)b * a.S + r / G) * a.H * D + (int64_t)(kvh * G + r % G) * D + 4 * (e % D4);
+    if (a.out) *reinterpret_cast<float4 *>(a.out + at) = acc;
+    if (a.out16) {
+      const __half2 h0 = __floats2half2_rn(acc.x, acc.y), h1 = __floats2half2_rn(acc.z, acc.w);
+      *reinterpret_cast<uint2 *>(a.out16 + at) = make_uint2(b2m::h2_as_u32(h0), b2m::h2_as_u32(h1));
+    }
+  }
+  if (CL > 1) cluster.sync();  // the others have read this CTA's state
+}
+
+template <bool E4M3, int D, int NT>
+void launch(const Kv8Args &a, cudaStream_t s) {
+  using M = StepSmem<D, NT>;
+  constexpr auto kern = kv8_step_kernel<E4M3, D, NT>;
+  b2m::set_smem_limit_once<kern>(M::BYTES);
+  const int nrows = a.S * (a.H / a.KVH), tiles = (nrows + M::R - 1) / M::R;
+  if (tiles > 1) launch_kv8_append(a, s);
+  // Key splits: CTAs for four per SM, at least 64 cache positions each.
+  const int64_t ctas = (int64_t)a.B * a.KVH * tiles;
+  int cl = 1;
+  while (cl < 8 && ctas * cl < 4 * b2m::device_sm_count() && a.CAP > 64 * cl) cl *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * cl), (unsigned)a.KVH, (unsigned)a.B);
+  cfg.blockDim = dim3(ST_THREADS);
+  cfg.dynamicSmemBytes = M::BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cl;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  B2M_CUDA(cudaLaunchKernelEx(&cfg, kern, a, tiles == 1 ? 1 : 0));
+}
+
+template <bool E4M3, int D>
+void launch_rows(const Kv8Args &a, cudaStream_t s) {
+  if (a.S * (a.H / a.KVH) <= 8)
+    launch<E4M3, D, 1>(a, s);
+  else
+    launch<E4M3, D, 2>(a, s);
+}
+
+template <bool E4M3>
+void launch_dim(const Kv8Args &a, cudaStream_t s) {
+  switch (a.D) {
+    case 32: return launch_rows<E4M3, 32>(a, s);
+    case 64: return launch_rows<E4M3, 64>(a, s);
+    case 96: return launch_rows<E4M3, 96>(a, s);
+    case 128: return launch_rows<E4M3, 128>(a, s);
+    default: return launch<E4M3, 256, 1>(a, s);
+  }
+}
+
+}  // namespace
+
+// Head dims the kernel is compiled for, cache rows it can copy 16 bytes at a
+// time, outputs it can store four values at a time.
+bool kv8_step_shape(const Kv8Args &a) {
+  auto al = [](const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  return (a.D == 32 || a.D == 64 || a.D == 96 || a.D == 128 || a.D == 256) && al(a.kc, 16) && al(a.vc, 16) &&
+         al(a.out, 16) && al(a.out16, 8) && a.KVH <= 65535;
+}
+
+void launch_kv8_step(const Kv8Args &a, cudaStream_t s) {
+  if (a.e4m3)
+    launch_dim<true>(a, s);
+  else
+    launch_dim<false>(a, s);
+}
