@@ -51,6 +51,18 @@ void set_smem_limit_once(int bytes) {
   done.fetch_or(bit, std::memory_order_acq_rel);
 }
 
+// Allows kernel Kern clusters of more than eight CTAs, once per device.
+template <auto Kern>
+void allow_large_cluster_once() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  B2M_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return;
+  B2M_CUDA(cudaFuncSetAttribute(Kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  done.fetch_or(bit, std::memory_order_acq_rel);
+}
+
 // x -> (x0, x1) = (rn_bf16(x), rn_bf16(x - x0)), the two-term split of the
 // FAST fp32 GEMM's operands. A finite x whose rounding overflows bf16 keeps
 // its truncation as x0; a non-finite x passes through x0.
