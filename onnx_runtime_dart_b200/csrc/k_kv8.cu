@@ -215,6 +215,11 @@ void launch_kv8_keep(const Kv8Args &a, int layers, const int32_t *path, const in
 }
 
 void launch_kv8_attend(const Kv8Args &a, bool exact, cudaStream_t s) {
+  if (!exact && kv8_flash_shape(a)) {
+    launch_kv8_append(a, s);
+    launch_kv8_flash(a, s);
+    return;
+  }
   if (!exact && kv8_step_shape(a)) {
     launch_kv8_step(a, s);
     return;

@@ -1,0 +1,657 @@
+// Attention over the 8-bit KV cache for many query rows per kv head (prompts,
+// chunks, wide drafted trees) on tcgen05; head_dim 64 or 128.
+//
+// A CTA takes 128 query rows of one (kv head, sequence): row r is query head
+// r % G of token r / G, so the heads of a group share the K / V tiles. Keys come
+// in tiles of 64. Roles:
+//   warps 4-7  expand a tile's codes (exact f16 numbers) into shared memory, K as
+//              [64 keys][D], V transposed as [D][64 keys] (128-byte swizzle), the
+//              next tile's codes already in flight in registers;
+//   warp 8     (of a third warpgroup) one thread issues S_j = Q . K_j^T (S in TMEM, two buffers) and
+//              O += P_j . V_j with P in TMEM as the A operand; S_{j+1} is issued
+//              before P_j is waited for, so the tensor cores work under the softmax;
+//   warps 0-3  a thread per query row (= TMEM lane): scores times K's scale,
+//              the causal or tree mask, exp2 against a reference that only moves
+//              when a score passes it by 2^5 (O in TMEM is rescaled then), the
+//              weights times V's scale as f16 back into S's columns.
+// No cross-thread reduction is left in the softmax. Two CTAs share an SM, so one's
+// exponentials run under the other's products.
+//
+// SPLIT (an fp32 output is wanted): Q and P as two f16 terms each, two products
+// per operand pair, fp32 accuracy. Without it Q and P are rounded to f16 once,
+// an error below that of the f16 output's own rounding.
+//
+// Few row tiles over many keys (a tree on long sequences): the CTAs of a cluster
+// split the keys and merge their O, m and l through distributed shared memory in
+// rank order; no workspace, no atomics.
+//
+// Every wait is bounded; one that gives up records the device error and all
+// roles leave their loops.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "kv8_common.cuh"
+#include "tc_common.cuh"
+
+namespace {
+
+namespace cg = cooperative_groups;
+using namespace kv8;
+using namespace b2m;
+
+constexpr int FL_THREADS = 384, FL_TILE = 64, FL_ROWS = 128, FL_SLOTS = 4;
+// Registers per thread: at launch (two CTAs per SM), then per role, and the
+// launch's number again for the common end. The CTA's three warpgroups share
+// what it was launched with: the roles' sum is no more.
+constexpr int FL_REGS = 80, FL_REGS_SOFTMAX = 144, FL_REGS_TILES = 72, FL_REGS_MMA = 24;
+static_assert(FL_REGS_SOFTMAX + FL_REGS_TILES + FL_REGS_MMA <= 3 * FL_REGS, "register split");
+constexpr float FL_BIAS = 10.f, FL_SLACK = 5.f;  // log2: weights stay below 2^15
+
+__device__ __forceinline__ uint32_t sw128(int r, int k) {  // byte offset of 16-bit element k < 64 of row r
+  return (uint32_t)(r * 128 + ((((k >> 3) ^ (r & 7)) << 4) | ((k & 7) << 1)));
+}
+
+template <int D, bool SPLIT>
+struct FlashLayout {
+  static constexpr int ND = D / 64;
+  static constexpr int KST = SPLIT ? 1 : 2, VST = SPLIT ? 1 : 2;
+  static constexpr uint32_t QH = 0, QL = ND * 16384;
+  static constexpr uint32_t K = QL + (SPLIT ? ND * 16384 : 0), K_STAGE = ND * 8192;
+  static constexpr uint32_t V = K + KST * K_STAGE, V_STAGE = D * 128;
+  static constexpr uint32_t TILES = V + VST * V_STAGE;
+  // O staging [128][D + 4] fp32 at the end, over Q, K and V
+  static constexpr int OST = D + 4;
+  static constexpr uint32_t SCALES0 = 128 * OST * 4 > TILES ? 128 * OST * 4 : TILES;
+  // ks[SLOTS][64], vs[SLOTS][64], vf[SLOTS], vref; then per row: factor, limit,
+  // bits, m, l; barriers
+  static constexpr uint32_t SCALES = SCALES0;
+  static constexpr uint32_t VF = SCALES + FL_SLOTS * 64 * 8, VREF = VF + FL_SLOTS * 4;
+  static constexpr uint32_t ROWS = VREF + 16;
+  static constexpr uint32_t BARS = ROWS + 128 * (8 + 4 + 4 + 4 + 4);
+  static constexpr uint32_t SLOT = BARS + 14 * 8, FLAG = SLOT + 4;
+  static constexpr uint32_t BYTES = FLAG + 4;
+  static constexpr uint32_t T_O = 128;  // TMEM: S / P buffers at 0 and 64, O at 128
+  static_assert(BYTES <= 113 * 1024, "two CTAs per SM");
+};
+
+template <bool E4M3, int D, bool SPLIT>
+__global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args a) {
+  using L = FlashLayout<D, SPLIT>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float *ks_s = reinterpret_cast<float *>(smem + L::SCALES), *vs_s = ks_s + FL_SLOTS * 64;
+  float *vf_s = reinterpret_cast<float *>(smem + L::VF), *vref_s = reinterpret_cast<float *>(smem + L::VREF);
+  uint64_t *row_bits = reinterpret_cast<uint64_t *>(smem + L::ROWS);
+  float *row_factor = reinterpret_cast<float *>(row_bits + 128);
+  int *row_lim = reinterpret_cast<int *>(row_factor + 128);
+  float *row_m = reinterpret_cast<float *>(row_lim + 128), *row_l = row_m + 128;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BARS);
+  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8,
+           *p_full = bars + 10, *o_done = bars + 12, *all_done = bars + 13;
+  uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::SLOT);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::FLAG);
+
+  pdl_launch_dependents();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int tiles = (int)(gridDim.x / CL);
+  const int row0 = (tiles - 1 - (int)(blockIdx.x / CL)) * FL_ROWS;  // the longest rows first
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int G = a.H / a.KVH, nrows = a.S * G;
+  const int past = max(0, a.past[b]);
+  const int last_token = min(a.S - 1, (row0 + FL_ROWS - 1) / G);
+  const int n = (int)min((int64_t)a.CAP, (int64_t)past + (a.tree ? a.S : last_token + 1));
+  const int all_tiles = (n + FL_TILE - 1) / FL_TILE, per = (all_tiles + CL - 1) / CL;
+  const int t0 = min(all_tiles, rank * per), ntile = min(all_tiles, t0 + per) - t0;
+  const int64_t base = ((int64_t)b * a.KVH + kvh) * a.CAP;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(k_full + i, 128);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_full + i, 128);
+      mbar_init(v_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 128);
+    }
+    mbar_init(o_done, 1);
+    mbar_init(all_done, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 8) tmem_alloc(slot, 256);
+
+  // Q rows, eight lanes each (lane l8 holds the float4 chunks l8 + 8 i): head
+  // norm, rotary, scaled by a power of two to a largest magnitude in [2^9, 2^10).
+  {
+    constexpr int NC = D / 32;  // chunks per lane
+    const int l8 = lane & 7;
+    for (int rr = warp * 4 + (lane >> 3); rr < FL_ROWS; rr += FL_THREADS / 8) {
+      const int r = row0 + rr;
+      const bool valid = r < nrows;
+      const int i = valid ? r / G : 0, h = kvh * G + (valid ? r % G : 0);
+      const float *src = a.q + ((int64_t)b * a.S + i) * a.q_rs + (int64_t)h * D;
+      const float *gain = a.q_gain ? a.q_gain + (int64_t)h * D : nullptr;
+      const int64_t pos = token_pos(a, b, i, past);
+      const bool turn = a.cos && pos >= 0 && pos < a.CAP;
+      const int hr = a.rot >> 1;
+      float4 v[NC];
+#pragma unroll
+      for (int u = 0; u < NC; u++) v[u] = *reinterpret_cast<const float4 *>(src + 4 * (l8 + 8 * u));
+      float inv = 1.f;
+      if (gain) {
+        float ss = 0.f;
+#pragma unroll
+        for (int u = 0; u < NC; u++)
+          ss = fmaf(v[u].x, v[u].x, fmaf(v[u].y, v[u].y, fmaf(v[u].z, v[u].z, fmaf(v[u].w, v[u].w, ss))));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        inv = 1.f / sqrtf(ss / D + (float)a.eps);
+      }
+      float mx = 0.f;
+#pragma unroll
+      for (int u = 0; u < NC; u++) {
+        const int d = 4 * (l8 + 8 * u);
+        float x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+        if (gain) {
+          const float4 g4 = *reinterpret_cast<const float4 *>(gain + d);
+          x[0] *= inv * g4.x, x[1] *= inv * g4.y, x[2] *= inv * g4.z, x[3] *= inv * g4.w;
+        }
+        if (turn && d < a.rot) {
+          // (the launcher takes rotary_dim % 8 == 0: a chunk and its partner are whole float4s)
+          const bool first = a.interleaved || d < hr;
+          float c[4], sn[4], w[4];
+          if (a.interleaved) {
+            const float2 c2 = *reinterpret_cast<const float2 *>(a.cos + pos * a.half + (d >> 1));
+            const float2 s2 = *reinterpret_cast<const float2 *>(a.sin + pos * a.half + (d >> 1));
+            c[0] = c[1] = c2.x, c[2] = c[3] = c2.y;
+            sn[0] = s2.x, sn[1] = -s2.x, sn[2] = s2.y, sn[3] = -s2.y;
+            w[0] = x[1], w[1] = x[0], w[2] = x[3], w[3] = x[2];
+          } else {
+            const int pi = first ? d : d - hr, e = first ? d + hr : d - hr;
+            const float4 c4 = *reinterpret_cast<const float4 *>(a.cos + pos * a.half + pi);
+            const float4 s4 = *reinterpret_cast<const float4 *>(a.sin + pos * a.half + pi);
+            float4 w4 = *reinterpret_cast<const float4 *>(src + e);
+            if (gain) {
+              const float4 g4 = *reinterpret_cast<const float4 *>(gain + e);
+              w4.x *= inv * g4.x, w4.y *= inv * g4.y, w4.z *= inv * g4.z, w4.w *= inv * g4.w;
+            }
+            c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w;
+            const float sg = first ? 1.f : -1.f;
+            sn[0] = sg * s4.x, sn[1] = sg * s4.y, sn[2] = sg * s4.z, sn[3] = sg * s4.w;
+            w[0] = w4.x, w[1] = w4.y, w[2] = w4.z, w[3] = w4.w;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; k++) x[k] = x[k] * c[k] - w[k] * sn[k];
+        }
+        v[u] = valid ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      // mx = f 2^e, f in [1/2, 1), times 2^(10 - e) in two steps (either may leave
+      // the normal range alone). Zero, infinite and NaN rows: any exponent does.
+      int e = 10;
+      if (mx > 0.f && mx < INFINITY) frexpf(mx, &e);
+      const int e1 = (10 - e) / 2, e2 = 10 - e - e1;
+      const float f1 = __uint_as_float((uint32_t)(127 + e1) << 23), f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
+#pragma unroll
+      for (int u = 0; u < NC; u++) {
+        const int d = 4 * (l8 + 8 * u);
+        const float4 x = make_float4(v[u].x * f1 * f2, v[u].y * f1 * f2, v[u].z * f1 * f2, v[u].w * f1 * f2);
+        const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
+        const uint32_t at = (uint32_t)(d >> 6) * 16384u + sw128(rr, d & 63);
+        *reinterpret_cast<uint2 *>(smem + L::QH + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
+        if (SPLIT) {
+          const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
+          *reinterpret_cast<uint2 *>(smem + L::QL + at) =
+              make_uint2(h2_as_u32(__floats2half2_rn(x.x - g0.x, x.y - g0.y)),
+                         h2_as_u32(__floats2half2_rn(x.z - g1.x, x.w - g1.y)));
+        }
+      }
+      if (l8 == 0) {
+        row_factor[rr] = ldexpf(a.scale * LOG2E * code_factor<E4M3>(), e - 10);
+        row_lim[rr] = !valid ? -1 : (a.tree ? past - 1 : past + i);
+        row_bits[rr] = valid && a.tree ? a.tree[(int64_t)b * a.S + i] : 0;
+      }
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+
+  if (warp >= 4 && warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FL_REGS_TILES));
+    // ---- K / V tiles -------------------------------------------------------
+    const int ct = tid - 128, cw = warp - 4;
+    constexpr int KI = 64 * (D / 16) / 128, VI = D / 64;  // 16-byte items per thread: K; V (per key of the pair)
+    uint4 kreg[KI], vreg[2][VI];
+    float sc[2];
+    const uint8_t *kc = a.kc + base * D, *vc = a.vc + base * D;
+    // K: eight lanes take eight rows of one 16-byte chunk (conflict-free stores)
+    auto k_item = [&](int u, int &row, int &c) {
+      const int it = ct + 128 * u;
+      row = (it & 7) + 8 * (it / (8 * (D / 16)));
+      c = (it >> 3) % (D / 16);
+    };
+    auto load_k = [&](int t) {
+      const int j0 = (t0 + t) * FL_TILE;
+#pragma unroll
+      for (int u = 0; u < KI; u++) {
+        int row, c;
+        k_item(u, row, c);
+        kreg[u] = *reinterpret_cast<const uint4 *>(kc + (int64_t)min(j0 + row, n - 1) * D + 16 * c);
+      }
+      // warps 0, 1: K's scales (one per lane); warps 2, 3: V's (two per lane)
+      if (cw < 2) {
+        sc[0] = a.ks[base + min(j0 + ct, n - 1)];
+      } else {
+        sc[0] = a.vs[base + min(j0 + lane, n - 1)];
+        sc[1] = a.vs[base + min(j0 + 32 + lane, n - 1)];
+      }
+    };
+    // V: lane p takes keys 2p, 2p + 1, warp w the chunks w VI ...
+    auto load_v = [&](int t) {
+      const int j0 = (t0 + t) * FL_TILE;
+#pragma unroll
+      for (int q = 0; q < 2; q++)
+#pragma unroll
+        for (int u = 0; u < VI; u++)
+          vreg[q][u] = *reinterpret_cast<const uint4 *>(vc + (int64_t)min(j0 + 2 * lane + q, n - 1) * D +
+                                                        16 * (cw * VI + u));
+    };
+    float vref = 0.f, vinv = 0.f;
+    if (ntile > 0) {
+      load_k(0);
+      load_v(0);
+    }
+    for (int t = 0; t < ntile; t++) {
+      const int kst = t % L::KST, vst = t % L::VST, sl = t % FL_SLOTS;
+      if (t >= L::KST && !wait_or_abort(k_empty + kst, (uint32_t)(t / L::KST - 1) & 1u, abort_flag, a.err)) break;
+      uint8_t *kd = smem + L::K + kst * L::K_STAGE;
+#pragma unroll
+      for (int u = 0; u < KI; u++) {
+        int row, c;
+        k_item(u, row, c);
+        const uint32_t w[4] = {kreg[u].x, kreg[u].y, kreg[u].z, kreg[u].w};
+        uint32_t o[8];
+#pragma unroll
+        for (int k = 0; k < 4; k++) expand4<E4M3>(w[k], o[2 * k], o[2 * k + 1]);
+        uint8_t *blk = kd + (c >> 2) * 8192;
+        *reinterpret_cast<uint4 *>(blk + sw128(row, (16 * c) & 63)) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4 *>(blk + sw128(row, ((16 * c) & 63) + 8)) = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+      if (cw < 2) {
+        ks_s[sl * 64 + ct] = sc[0];
+      } else {
+        // V's scales over the power of two above the largest so far (both warps
+        // come to the same one); a change tells the softmax to rescale O.
+        float vm = fmaxf(sc[0], sc[1]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+        float vf = 1.f;
+        if (vm > vref) {
+          const float up = __uint_as_float(min(max((__float_as_uint(vm) >> 23) + 1u, 2u), 252u) << 23);
+          vinv = 1.f / up;
+          vf = vref * vinv;
+          vref = up;
+        }
+        if (cw == 2)
+          vs_s[sl * 64 + lane] = sc[0] * vinv;
+        else
+          vs_s[sl * 64 + 32 + lane] = sc[1] * vinv;
+        if (cw == 2 && lane == 0) {
+          vf_s[sl] = vf;
+          *vref_s = vref;
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(k_full + kst);
+      if (t + 1 < ntile) load_k(t + 1);
+      if (t >= L::VST && !wait_or_abort(v_empty + vst, (uint32_t)(t / L::VST - 1) & 1u, abort_flag, a.err)) break;
+      uint8_t *vd = smem + L::V + vst * L::V_STAGE;
+#pragma unroll
+      for (int u = 0; u < VI; u++) {
+        const uint32_t w0[4] = {vreg[0][u].x, vreg[0][u].y, vreg[0][u].z, vreg[0][u].w};
+        const uint32_t w1[4] = {vreg[1][u].x, vreg[1][u].y, vreg[1][u].z, vreg[1][u].w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          uint32_t o[4];  // dims 4k .. 4k+3: keys (2p, 2p+1)
+          expand4<E4M3>(prmt(w0[k], w1[k], PAIR01), o[0], o[1]);
+          expand4<E4M3>(prmt(w0[k], w1[k], PAIR23), o[2], o[3]);
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            *reinterpret_cast<uint32_t *>(vd + sw128(16 * (cw * VI + u) + 4 * k + e, 2 * lane)) = o[e];
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(v_full + vst);
+      if (t + 1 < ntile) load_v(t + 1);
+    }
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FL_REGS_MMA));
+    // ---- tensor cores ------------------------------------------------------
+    if (warp == 8 && lane == 0 && ntile > 0) {
+      constexpr uint32_t idesc_s = umma_idesc(128, FL_TILE, 1u, 0u, 0u), idesc_o = umma_idesc(128, D, 1u, 0u, 0u);
+      const uint32_t sb = smem_u32(smem);
+      const uint64_t d_qh = sw128_kmajor_desc(sb + L::QH), d_ql = sw128_kmajor_desc(sb + L::QL);
+      auto issue_s = [&](int t) {
+        const uint64_t dk = sw128_kmajor_desc(sb + L::K + (t % L::KST) * L::K_STAGE);
+        const uint32_t ts = tmem + (uint32_t)(t & 1) * 64u;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; kk++) {
+          const uint64_t oq = ((kk >> 2) * 16384u + (kk & 3) * 32u) >> 4, ok = ((kk >> 2) * 8192u + (kk & 3) * 32u) >> 4;
+          if (SPLIT) umma_f16(ts, d_ql + oq, dk + ok, idesc_s, kk ? 1u : 0u);
+          umma_f16(ts, d_qh + oq, dk + ok, idesc_s, SPLIT || kk ? 1u : 0u);
+        }
+        umma_commit(s_full + (t & 1));
+        umma_commit(k_empty + t % L::KST);
+      };
+      bool ok = wait_or_abort(k_full, 0u, abort_flag, a.err);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0);
+      }
+      for (int t = 0; ok && t < ntile; t++) {
+        if (t + 1 < ntile) {
+          const int st = (t + 1) % L::KST;
+          // S_{t+1} takes the columns of P_{t-1}: products of different shapes are
+          // not ordered among themselves, so P_{t-1} . V must be through.
+          ok = (t == 0 || wait_or_abort(o_done, (uint32_t)(t - 1) & 1u, abort_flag, a.err)) &&
+               wait_or_abort(k_full + st, (uint32_t)((t + 1) / L::KST) & 1u, abort_flag, a.err);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(t + 1);
+        }
+        ok = wait_or_abort(v_full + t % L::VST, (uint32_t)(t / L::VST) & 1u, abort_flag, a.err) &&
+             wait_or_abort(p_full + (t & 1), (uint32_t)(t >> 1) & 1u, abort_flag, a.err);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t dv = sw128_kmajor_desc(sb + L::V + (t % L::VST) * L::V_STAGE);
+        const uint32_t tp = tmem + (uint32_t)(t & 1) * 64u;
+#pragma unroll
+        for (int kk = 0; kk < FL_TILE / 16; kk++) {
+          const uint64_t ov = (kk * 32u) >> 4;
+          if (SPLIT) umma_f16_ts(tmem + L::T_O, tp + 32u + 8u * kk, dv + ov, idesc_o, t || kk ? 1u : 0u);
+          umma_f16_ts(tmem + L::T_O, tp + 8u * kk, dv + ov, idesc_o, SPLIT || t || kk ? 1u : 0u);
+        }
+        umma_commit(v_empty + t % L::VST);
+        umma_commit(o_done);
+        // A barrier of its own for the last one: a waiter that has not seen the
+        // phase before could take o_done's parity for the one it waits for. (In the
+        // loop S_t is there, and S_t was issued behind phase t - 2.)
+        if (t + 1 == ntile) umma_commit(all_done);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FL_REGS_SOFTMAX));
+    // ---- softmax -----------------------------------------------------------
+    const int rr = tid;
+    const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
+    const float rf = row_factor[rr];
+    const int lim = row_lim[rr];
+    const uint64_t bits = row_bits[rr];
+    const int all_see = a.tree ? past : past + row0 / G + 1;  // keys below this are seen by every row
+    float m = -INFINITY, mref = 0.f, l = 0.f;
+    bool ok = true;
+    for (int t = 0; t < ntile; t++) {
+      const int sl = t % FL_SLOTS, j0 = (t0 + t) * FL_TILE;
+      ok = warp_wait_or_abort(s_full + (t & 1), (uint32_t)(t >> 1) & 1u, abort_flag, a.err);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t ts = trow + (uint32_t)(t & 1) * 64u;
+      float x[FL_TILE];
+      {
+        uint32_t u[4][16];
+#pragma unroll
+        for (int c = 0; c < 4; c++) tmem_ld16(ts + 16u * c, u[c]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < FL_TILE; c++) x[c] = __uint_as_float(u[c >> 4][c & 15]);
+      }
+      const float4 *kp = reinterpret_cast<const float4 *>(ks_s + sl * 64);
+#pragma unroll
+      for (int c = 0; c < FL_TILE / 4; c++) {
+        const float4 k4 = kp[c];
+        x[4 * c] *= k4.x, x[4 * c + 1] *= k4.y, x[4 * c + 2] *= k4.z, x[4 * c + 3] *= k4.w;
+      }
+      const bool whole = j0 + FL_TILE <= min(n, all_see);
+      uint64_t seen = ~0ull;
+      if (!whole) {
+        // Bit c: key j0 + c. Causal (and cached) keys up to lim; tree bits from past on.
+        const int below = min(lim + 1, n) - j0;
+        seen = below >= 64 ? ~0ull : (below <= 0 ? 0ull : (1ull << below) - 1);
+        if (a.tree) {
+          const int sh = past - j0;  // the tree's bit 0 is key j0 + sh
+          uint64_t tb = sh >= 64 || sh <= -64 ? 0ull : (sh >= 0 ? bits << sh : bits >> -sh);
+          const int end = n - j0;
+          if (end < 64) tb &= end <= 0 ? 0ull : (1ull << end) - 1;
+          seen |= tb;
+        }
+#pragma unroll
+        for (int c = 0; c < FL_TILE; c++)
+          if (!(seen >> c & 1)) x[c] = -INFINITY;
+      }
+      float xm = x[0];
+#pragma unroll
+      for (int c = 1; c < FL_TILE; c++) xm = fmaxf(xm, x[c]);
+      xm *= rf;  // rf > 0; -inf stays
+      const float vf = vf_s[sl];
+      if (__any_sync(0xffffffffu, xm > m + FL_SLACK || vf != 1.f)) {
+        const float mn = fmaxf(m, xm);
+        float f = vf;
+        if (mn > m) {
+          const float fm = m == -INFINITY ? 0.f : ex2(m - mn);
+          l = l == 0.f ? 0.f : l * fm;
+          f *= fm;
+          m = mn;
+          mref = mn - FL_BIAS;
+        }
+        if (t > 0) {  // O holds the tiles before: rescale it once their products are done
+          ok = warp_wait_or_abort(o_done, (uint32_t)(t - 1) & 1u, abort_flag, a.err);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; c++) {
+            uint32_t u0[16], u1[16], w[32];
+            tmem_ld16(trow + L::T_O + 32u * c, u0);
+            tmem_ld16(trow + L::T_O + 32u * c + 16u, u1);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+              w[k] = __float_as_uint(__uint_as_float(u0[k]) * f);
+              w[16 + k] = __float_as_uint(__uint_as_float(u1[k]) * f);
+            }
+            tmem_st32(trow + L::T_O + 32u * c, w);
+          }
+          tmem_st_wait();
+        }
+      }
+      const float4 *vp = reinterpret_cast<const float4 *>(vs_s + sl * 64);
+      uint32_t ph[32], pl[SPLIT ? 32 : 1];
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < FL_TILE / 4; c++) {
+        const float4 v4 = vp[c];
+        const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
+        float w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float p = ex2(fmaf(x[4 * c + k], rf, -mref));
+          sum += p;
+          w[k] = p * vv[k];
+        }
+        if (!whole) {  // a hidden key's scale may be NaN
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            if (!(seen >> (4 * c + k) & 1)) w[k] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const __half2 h = __floats2half2_rn(w[2 * k], w[2 * k + 1]);
+          ph[2 * c + k] = h2_as_u32(h);
+          if (SPLIT) {
+            const float2 g = __half22float2(h);
+            pl[SPLIT ? 2 * c + k : 0] = h2_as_u32(__floats2half2_rn(w[2 * k] - g.x, w[2 * k + 1] - g.y));
+          }
+        }
+      }
+      l += sum;
+      tmem_st32(ts, ph);
+      if constexpr (SPLIT) tmem_st32(ts + 32u, pl);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_full + (t & 1));  // two: a warp may be a tile ahead of another (S_{t+1} is there early)
+    }
+    if (ok && ntile > 0) ok = warp_wait_or_abort(all_done, 0u, abort_flag, a.err);
+    tc_fence_after();
+    // O (in the values' own scale), m and l to shared memory: Q, K and V are no
+    // longer read (the last products have completed).
+    float *ost = reinterpret_cast<float *>(smem) + rr * L::OST;
+    if (ok) {
+      const float vo = ntile > 0 ? *vref_s * code_factor<E4M3>() : 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 16; c++) {
+        uint32_t u[16];
+        if (ntile > 0) {
+          tmem_ld16(trow + L::T_O + 16u * c, u);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int k = 0; k < 16; k += 4)
+          *reinterpret_cast<float4 *>(ost + 16 * c + k) =
+              ntile > 0 ? make_float4(__uint_as_float(u[k]) * vo, __uint_as_float(u[k + 1]) * vo,
+                                      __uint_as_float(u[k + 2]) * vo, __uint_as_float(u[k + 3]) * vo)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    row_m[rr] = m;
+    row_l[rr] = l;
+  }
+  // All roles meet before any takes registers back: a warp that gave its up and
+  // took them again at once could leave the softmax waiting for its share. Behind
+  // the barrier the softmax gives, the others take, and none waits for another.
+  tc_fence_before();
+  __syncthreads();
+  __syncwarp();
+  if (warp < 4)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FL_REGS));
+  else
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FL_REGS));
+  if (CL > 1) cluster.sync();
+  // Rows to memory, a cluster's ranks sharing them.
+  const float *o_s = reinterpret_cast<const float *>(smem);
+  constexpr int D4 = D / 4;
+  for (int e = rank * FL_THREADS + tid; e < FL_ROWS * D4; e += CL * FL_THREADS) {
+    const int rr = e / D4, c = e % D4, r = row0 + rr;
+    if (r >= nrows || *abort_flag) continue;
+    const float *src = o_s + rr * L::OST + 4 * c;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    if (CL == 1) {
+      acc = *reinterpret_cast<const float4 *>(src);
+      sum = row_l[rr];
+    } else {
+      float top = -INFINITY;
+      for (int q = 0; q < CL; q++) top = fmaxf(top, *cluster.map_shared_rank(row_m + rr, q));
+      for (int q = 0; q < CL; q++) {
+        const float sl = *cluster.map_shared_rank(row_l + rr, q), sm = *cluster.map_shared_rank(row_m + rr, q);
+        // none if that rank saw no key; with a NaN sum and no maximum the NaN is passed on
+        const float f = sl == 0.f ? 0.f : (sm == -INFINITY ? 1.f : ex2(sm - top));
+        const float4 v = *cluster.map_shared_rank(reinterpret_cast<const float4 *>(src), q);
+        sum += sl * f;
+        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that saw nothing: zeros
+    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+    const int64_t at = ((int64_t)b * a.S + r / G) * a.H * D + (int64_t)(kvh * G + r % G) * D + 4 * c;
+    if (a.out) *reinterpret_cast<float4 *>(a.out + at) = acc;
+    if (a.out16) {
+      const __half2 h0 = __floats2half2_rn(acc.x, acc.y), h1 = __floats2half2_rn(acc.z, acc.w);
+      *reinterpret_cast<uint2 *>(a.out16 + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
+    }
+  }
+  if (CL > 1) cluster.sync();  // the others have read this CTA's rows
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+// The register split needs what the kernel was designed to be launched with: a
+// build with fewer would wait for registers that are not there.
+template <auto Kern>
+void require_regs_once() {
+  static std::atomic<int> regs{0};
+  if (regs.load(std::memory_order_acquire) == 0) {
+    cudaFuncAttributes at;
+    B2M_CUDA(cudaFuncGetAttributes(&at, Kern));
+    regs.store(at.numRegs, std::memory_order_release);
+  }
+  B2M_REQUIRE(regs.load(std::memory_order_acquire) >= FL_REGS, B2M_ERR_UNSUPPORTED,
+              "GroupQueryAttention (8-bit cache): the flash kernel was built with another register count");
+}
+
+template <bool E4M3, int D, bool SPLIT>
+void launch(const Kv8Args &a, cudaStream_t s) {
+  using L = FlashLayout<D, SPLIT>;
+  constexpr auto kern = kv8_flash_kernel<E4M3, D, SPLIT>;
+  set_smem_limit_once<kern>((int)L::BYTES);
+  require_regs_once<kern>();
+  const int nrows = a.S * (a.H / a.KVH), tiles = (nrows + FL_ROWS - 1) / FL_ROWS;
+  // Key splits until two CTAs per SM are there, each with two tiles or more.
+  const int64_t ctas = (int64_t)a.B * a.KVH * tiles;
+  int cl = 1;
+  while (cl < 8 && ctas * cl * 2 <= 2 * device_sm_count() && a.CAP > 2 * FL_TILE * cl) cl *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * cl), (unsigned)a.KVH, (unsigned)a.B);
+  cfg.blockDim = dim3(FL_THREADS);
+  cfg.dynamicSmemBytes = L::BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cl;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  B2M_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+}
+
+template <bool E4M3, int D>
+void launch_out(const Kv8Args &a, cudaStream_t s) {
+  if (a.out)
+    launch<E4M3, D, true>(a, s);
+  else
+    launch<E4M3, D, false>(a, s);
+}
+
+}  // namespace
+
+// Enough rows to fill most of a 128-row tile; head dims, alignments and rotary
+// widths whose float4 chunks the prologue can take.
+bool kv8_flash_shape(const Kv8Args &a) {
+  auto al = [](const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  const int64_t rows = (int64_t)a.S * (a.H / a.KVH);
+  return (a.D == 64 || a.D == 128) && rows > 48 && rows < (1 << 30) && a.KVH <= 65535 && a.q_rs % 4 == 0 &&
+         al(a.q, 16) && al(a.kc, 16) && al(a.vc, 16) && al(a.out, 16) && al(a.out16, 8) && al(a.q_gain, 16) &&
+         (!a.cos || (a.rot % 8 == 0 && a.half % 4 == 0 && al(a.cos, 16) && al(a.sin, 16)));
+}
+
+// The call's keys and values must have been appended.
+void launch_kv8_flash(const Kv8Args &a, cudaStream_t s) {
+  if (a.e4m3) {
+    if (a.D == 128)
+      launch_out<true, 128>(a, s);
+    else
+      launch_out<true, 64>(a, s);
+  } else {
+    if (a.D == 128)
+      launch_out<false, 128>(a, s);
+    else
+      launch_out<false, 64>(a, s);
+  }
+}

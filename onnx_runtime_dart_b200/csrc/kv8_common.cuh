@@ -180,3 +180,6 @@ __host__ __device__ constexpr float code_factor() {
 // (k_kv8_step.cu).
 bool kv8_step_shape(const Kv8Args &a);
 void launch_kv8_step(const Kv8Args &a, cudaStream_t s);
+// The tcgen05 kernel for many rows (k_kv8_flash.cu), after launch_kv8_append.
+bool kv8_flash_shape(const Kv8Args &a);
+void launch_kv8_flash(const Kv8Args &a, cudaStream_t s);
