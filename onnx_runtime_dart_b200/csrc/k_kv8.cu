@@ -26,6 +26,18 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const Kv8Args a) {
   append_row(a, b, i, kvh, side, a.past[b], stage[warp], lane);
 }
 
+// The same for rows of whole float4s: one warp per (token, kv head), both sides.
+template <bool E4M3, int NCH>
+__global__ void __launch_bounds__(256) kv8_append_vec_kernel(const Kv8Args a) {
+  pdl_launch_dependents();
+  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned item = blockIdx.x * 8 + warp;  // (token, kv head): the launcher keeps it below 2^31
+  const unsigned i = item / (unsigned)a.KVH;
+  if (i >= (unsigned)a.S) return;
+  const int b = blockIdx.y;
+  append_pair_vec<E4M3, NCH>(a, b, (int)i, (int)(item - i * a.KVH), a.past[b], (int)lane);
+}
+
 // The values of n cached positions from start[b] (or 0) on, [B][KVH][n][D]
 // fp32: one warp per row.
 template <bool E4M3>
@@ -193,6 +205,22 @@ unsigned blocks_for(int64_t items, int per) {
 void launch_kv8_append(const Kv8Args &a, cudaStream_t s) {
   const int64_t items = (int64_t)a.B * a.S * a.KVH * 2;
   if (items == 0) return;
+  if (append_rows_vec(a) && (int64_t)a.S * a.KVH < ((int64_t)1 << 31) && a.B <= 65535) {
+    const dim3 grid((unsigned)(((int64_t)a.S * a.KVH + 7) / 8), (unsigned)a.B);
+    if (a.D <= 128) {
+      if (a.e4m3)
+        kv8_append_vec_kernel<true, 1><<<grid, 256, 0, s>>>(a);
+      else
+        kv8_append_vec_kernel<false, 1><<<grid, 256, 0, s>>>(a);
+    } else {
+      if (a.e4m3)
+        kv8_append_vec_kernel<true, 2><<<grid, 256, 0, s>>>(a);
+      else
+        kv8_append_vec_kernel<false, 2><<<grid, 256, 0, s>>>(a);
+    }
+    B2M_CUDA(cudaGetLastError());
+    return;
+  }
   kv8_append_kernel<<<blocks_for(items, 8), 256, 0, s>>>(a);
   B2M_CUDA(cudaGetLastError());
 }

@@ -44,12 +44,94 @@ constexpr int FL_THREADS = 384, FL_TILE = 64, FL_ROWS = 128, FL_SLOTS = 4;
 // Registers per thread: at launch (two CTAs per SM), then per role, and the
 // launch's number again for the common end. The CTA's three warpgroups share
 // what it was launched with: the roles' sum is no more.
-constexpr int FL_REGS = 80, FL_REGS_SOFTMAX = 144, FL_REGS_TILES = 72, FL_REGS_MMA = 24;
+constexpr int FL_REGS = 80, FL_REGS_SOFTMAX = 136, FL_REGS_TILES = 64, FL_REGS_MMA = 40;
 static_assert(FL_REGS_SOFTMAX + FL_REGS_TILES + FL_REGS_MMA <= 3 * FL_REGS, "register split");
 constexpr float FL_BIAS = 10.f, FL_SLACK = 5.f;  // log2: weights stay below 2^15
 
 __device__ __forceinline__ uint32_t sw128(int r, int k) {  // byte offset of 16-bit element k < 64 of row r
   return (uint32_t)(r * 128 + ((((k >> 3) ^ (r & 7)) << 4) | ((k & 7) << 1)));
+}
+
+// True in one lane of a converged warp. Code behind it may keep its addresses and
+// descriptors in uniform registers, where tcgen05.mma takes them from; behind a
+// test of the lane number each would be moved there first (100 cycles a product).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Two fp32 operations per instruction on register pairs.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 32 lanes x 32 consecutive 32-bit TMEM columns -> 16 register pairs per thread.
+__device__ __forceinline__ void tmem_ld32x2(uint32_t taddr, f32x2 *v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; i++) v[i] = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+}
+
+// Waits for phase `parity` of a barrier, suspended in the hardware for up to a
+// millisecond per try: at two CTAs per SM a dozen warps wait at any time, and
+// polling took half of the issue slots. Gives up when another thread has, or
+// after two seconds (and records the error).
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int32_t *dev_err) {
+  for (int i = 0; i < 2000; i++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+  }
+  *abort_flag = 1;
+  if (dev_err) set_dev_error(dev_err, B2M_DEVERR_MBAR_TIMEOUT);
+  return false;
+}
+// The same for a whole warp, one verdict for all lanes.
+__device__ __forceinline__ bool warp_wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort_flag,
+                                                int32_t *dev_err) {
+  return __all_sync(0xffffffffu, wait_phase(bar, parity, abort_flag, dev_err));
 }
 
 template <int D, bool SPLIT>
@@ -63,10 +145,10 @@ struct FlashLayout {
   // O staging [128][D + 4] fp32 at the end, over Q, K and V
   static constexpr int OST = D + 4;
   static constexpr uint32_t SCALES0 = 128 * OST * 4 > TILES ? 128 * OST * 4 : TILES;
-  // ks[SLOTS][64], vs[SLOTS][64], vf[SLOTS], vref; then per row: factor, limit,
+  // ks[SLOTS][64], vs[SLOTS][64], vf[SLOTS], vnan[SLOTS], vref; then per row: factor, limit,
   // bits, m, l; barriers
   static constexpr uint32_t SCALES = SCALES0;
-  static constexpr uint32_t VF = SCALES + FL_SLOTS * 64 * 8, VREF = VF + FL_SLOTS * 4;
+  static constexpr uint32_t VF = SCALES + FL_SLOTS * 64 * 8, VNAN = VF + FL_SLOTS * 4, VREF = VNAN + FL_SLOTS * 4;
   static constexpr uint32_t ROWS = VREF + 16;
   static constexpr uint32_t BARS = ROWS + 128 * (8 + 4 + 4 + 4 + 4);
   static constexpr uint32_t SLOT = BARS + 14 * 8, FLAG = SLOT + 4;
@@ -81,6 +163,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   extern __shared__ __align__(1024) uint8_t smem[];
   float *ks_s = reinterpret_cast<float *>(smem + L::SCALES), *vs_s = ks_s + FL_SLOTS * 64;
   float *vf_s = reinterpret_cast<float *>(smem + L::VF), *vref_s = reinterpret_cast<float *>(smem + L::VREF);
+  int *vnan_s = reinterpret_cast<int *>(smem + L::VNAN);
   uint64_t *row_bits = reinterpret_cast<uint64_t *>(smem + L::ROWS);
   float *row_factor = reinterpret_cast<float *>(row_bits + 128);
   int *row_lim = reinterpret_cast<int *>(row_factor + 128);
@@ -94,10 +177,9 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   pdl_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
-  const int tiles = (int)(gridDim.x / CL);
-  const int row0 = (tiles - 1 - (int)(blockIdx.x / CL)) * FL_ROWS;  // the longest rows first
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int row0 = (int)(gridDim.z - 1 - blockIdx.z) * FL_ROWS;  // the longest rows of all first
+  const int kvh = (int)(blockIdx.x / CL), b = blockIdx.y;
   const int G = a.H / a.KVH, nrows = a.S * G;
   const int past = max(0, a.past[b]);
   const int last_token = min(a.S - 1, (row0 + FL_ROWS - 1) / G);
@@ -221,7 +303,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *slot, 0);
 
   if (warp >= 4 && warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FL_REGS_TILES));
@@ -264,13 +346,10 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
                                                         16 * (cw * VI + u));
     };
     float vref = 0.f, vinv = 0.f;
-    if (ntile > 0) {
-      load_k(0);
-      load_v(0);
-    }
-    for (int t = 0; t < ntile; t++) {
-      const int kst = t % L::KST, vst = t % L::VST, sl = t % FL_SLOTS;
-      if (t >= L::KST && !wait_or_abort(k_empty + kst, (uint32_t)(t / L::KST - 1) & 1u, abort_flag, a.err)) break;
+    auto put_k = [&](int t) {
+      const int kst = t % L::KST, sl = t % FL_SLOTS;
+      if (t >= L::KST && !warp_wait_phase(k_empty + kst, (uint32_t)(t / L::KST - 1) & 1u, abort_flag, a.err))
+        return false;
       uint8_t *kd = smem + L::K + kst * L::K_STAGE;
 #pragma unroll
       for (int u = 0; u < KI; u++) {
@@ -303,15 +382,31 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           vs_s[sl * 64 + lane] = sc[0] * vinv;
         else
           vs_s[sl * 64 + 32 + lane] = sc[1] * vinv;
+        const bool nan = __any_sync(0xffffffffu, sc[0] != sc[0] || sc[1] != sc[1]);
         if (cw == 2 && lane == 0) {
+          vnan_s[sl] = nan;
           vf_s[sl] = vf;
           *vref_s = vref;
         }
       }
       fence_proxy_async_smem();
       mbar_arrive(k_full + kst);
-      if (t + 1 < ntile) load_k(t + 1);
-      if (t >= L::VST && !wait_or_abort(v_empty + vst, (uint32_t)(t / L::VST - 1) & 1u, abort_flag, a.err)) break;
+      return true;
+    };
+    if (ntile > 0) {
+      load_k(0);
+      load_v(0);
+      put_k(0);
+      if (ntile > 1) load_k(1);
+    }
+    // K_{t+1} before V_t: its products are wanted first (under tile t's softmax).
+    for (int t = 0; t < ntile; t++) {
+      if (t + 1 < ntile) {
+        if (!put_k(t + 1)) break;
+        if (t + 2 < ntile) load_k(t + 2);
+      }
+      const int vst = t % L::VST;
+      if (t >= L::VST && !warp_wait_phase(v_empty + vst, (uint32_t)(t / L::VST - 1) & 1u, abort_flag, a.err)) break;
       uint8_t *vd = smem + L::V + vst * L::V_STAGE;
 #pragma unroll
       for (int u = 0; u < VI; u++) {
@@ -334,7 +429,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FL_REGS_MMA));
     // ---- tensor cores ------------------------------------------------------
-    if (warp == 8 && lane == 0 && ntile > 0) {
+    if (warp == 8 && ntile > 0 && elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc(128, FL_TILE, 1u, 0u, 0u), idesc_o = umma_idesc(128, D, 1u, 0u, 0u);
       const uint32_t sb = smem_u32(smem);
       const uint64_t d_qh = sw128_kmajor_desc(sb + L::QH), d_ql = sw128_kmajor_desc(sb + L::QL);
@@ -350,7 +445,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         umma_commit(s_full + (t & 1));
         umma_commit(k_empty + t % L::KST);
       };
-      bool ok = wait_or_abort(k_full, 0u, abort_flag, a.err);
+      bool ok = wait_phase(k_full, 0u, abort_flag, a.err);
       if (ok) {
         tc_fence_after();
         issue_s(0);
@@ -360,14 +455,14 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           const int st = (t + 1) % L::KST;
           // S_{t+1} takes the columns of P_{t-1}: products of different shapes are
           // not ordered among themselves, so P_{t-1} . V must be through.
-          ok = (t == 0 || wait_or_abort(o_done, (uint32_t)(t - 1) & 1u, abort_flag, a.err)) &&
-               wait_or_abort(k_full + st, (uint32_t)((t + 1) / L::KST) & 1u, abort_flag, a.err);
+          ok = (t == 0 || wait_phase(o_done, (uint32_t)(t - 1) & 1u, abort_flag, a.err)) &&
+               wait_phase(k_full + st, (uint32_t)((t + 1) / L::KST) & 1u, abort_flag, a.err);
           if (!ok) break;
           tc_fence_after();
           issue_s(t + 1);
         }
-        ok = wait_or_abort(v_full + t % L::VST, (uint32_t)(t / L::VST) & 1u, abort_flag, a.err) &&
-             wait_or_abort(p_full + (t & 1), (uint32_t)(t >> 1) & 1u, abort_flag, a.err);
+        ok = wait_phase(v_full + t % L::VST, (uint32_t)(t / L::VST) & 1u, abort_flag, a.err) &&
+             wait_phase(p_full + (t & 1), (uint32_t)(t >> 1) & 1u, abort_flag, a.err);
         if (!ok) break;
         tc_fence_after();
         const uint64_t dv = sw128_kmajor_desc(sb + L::V + (t % L::VST) * L::V_STAGE);
@@ -399,24 +494,21 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     bool ok = true;
     for (int t = 0; t < ntile; t++) {
       const int sl = t % FL_SLOTS, j0 = (t0 + t) * FL_TILE;
-      ok = warp_wait_or_abort(s_full + (t & 1), (uint32_t)(t >> 1) & 1u, abort_flag, a.err);
+      ok = warp_wait_phase(s_full + (t & 1), (uint32_t)(t >> 1) & 1u, abort_flag, a.err);
       if (!ok) break;
       tc_fence_after();
       const uint32_t ts = trow + (uint32_t)(t & 1) * 64u;
-      float x[FL_TILE];
-      {
-        uint32_t u[4][16];
-#pragma unroll
-        for (int c = 0; c < 4; c++) tmem_ld16(ts + 16u * c, u[c]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < FL_TILE; c++) x[c] = __uint_as_float(u[c >> 4][c & 15]);
-      }
-      const float4 *kp = reinterpret_cast<const float4 *>(ks_s + sl * 64);
+      // Scores of the row's 64 keys as 32 pairs, times K's scales.
+      f32x2 x[FL_TILE / 2];
+      tmem_ld32x2(ts, x);
+      tmem_ld32x2(ts + 32u, x + 16);
+      tmem_ld_wait();
+      const ulonglong2 *kp = reinterpret_cast<const ulonglong2 *>(ks_s + sl * 64);
 #pragma unroll
       for (int c = 0; c < FL_TILE / 4; c++) {
-        const float4 k4 = kp[c];
-        x[4 * c] *= k4.x, x[4 * c + 1] *= k4.y, x[4 * c + 2] *= k4.z, x[4 * c + 3] *= k4.w;
+        const ulonglong2 k4 = kp[c];
+        x[2 * c] = mul2(x[2 * c], k4.x);
+        x[2 * c + 1] = mul2(x[2 * c + 1], k4.y);
       }
       const bool whole = j0 + FL_TILE <= min(n, all_see);
       uint64_t seen = ~0ull;
@@ -431,14 +523,28 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           if (end < 64) tb &= end <= 0 ? 0ull : (1ull << end) - 1;
           seen |= tb;
         }
+        const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
 #pragma unroll
-        for (int c = 0; c < FL_TILE; c++)
-          if (!(seen >> c & 1)) x[c] = -INFINITY;
+        for (int c = 0; c < FL_TILE / 2; c++) {
+          float x0, x1;
+          unpack2(x[c], x0, x1);
+          const uint32_t w = c < 16 ? s0 : s1;
+          x0 = w >> (2 * c & 31) & 1 ? x0 : -INFINITY;
+          x1 = w >> (2 * c + 1 & 31) & 1 ? x1 : -INFINITY;
+          x[c] = pack2(x0, x1);
+        }
       }
-      float xm = x[0];
+      float xm;
+      {
+        float q[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 1; c < FL_TILE; c++) xm = fmaxf(xm, x[c]);
-      xm *= rf;  // rf > 0; -inf stays
+        for (int c = 0; c < FL_TILE / 2; c++) {
+          float x0, x1;
+          unpack2(x[c], x0, x1);
+          q[c & 3] = max3(q[c & 3], x0, x1);
+        }
+        xm = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3])) * rf;  // rf > 0; -inf stays
+      }
       const float vf = vf_s[sl];
       if (__any_sync(0xffffffffu, xm > m + FL_SLACK || vf != 1.f)) {
         const float mn = fmaxf(m, xm);
@@ -451,62 +557,74 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           mref = mn - FL_BIAS;
         }
         if (t > 0) {  // O holds the tiles before: rescale it once their products are done
-          ok = warp_wait_or_abort(o_done, (uint32_t)(t - 1) & 1u, abort_flag, a.err);
+          ok = warp_wait_phase(o_done, (uint32_t)(t - 1) & 1u, abort_flag, a.err);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < D / 32; c++) {
-            uint32_t u0[16], u1[16], w[32];
-            tmem_ld16(trow + L::T_O + 32u * c, u0);
-            tmem_ld16(trow + L::T_O + 32u * c + 16u, u1);
+            f32x2 u[16];
+            uint32_t w[32];
+            tmem_ld32x2(trow + L::T_O + 32u * c, u);
             tmem_ld_wait();
 #pragma unroll
             for (int k = 0; k < 16; k++) {
-              w[k] = __float_as_uint(__uint_as_float(u0[k]) * f);
-              w[16 + k] = __float_as_uint(__uint_as_float(u1[k]) * f);
+              float u0, u1;
+              unpack2(u[k], u0, u1);
+              w[2 * k] = __float_as_uint(u0 * f);
+              w[2 * k + 1] = __float_as_uint(u1 * f);
             }
             tmem_st32(trow + L::T_O + 32u * c, w);
           }
           tmem_st_wait();
         }
       }
-      const float4 *vp = reinterpret_cast<const float4 *>(vs_s + sl * 64);
+      const ulonglong2 *vp = reinterpret_cast<const ulonglong2 *>(vs_s + sl * 64);
+      const f32x2 rf2 = pack2(rf, rf), mr2 = pack2(-mref, -mref);
       uint32_t ph[32], pl[SPLIT ? 32 : 1];
-      float sum = 0.f;
+      f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < FL_TILE / 4; c++) {
-        const float4 v4 = vp[c];
-        const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
-        float w[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const float p = ex2(fmaf(x[4 * c + k], rf, -mref));
-          sum += p;
-          w[k] = p * vv[k];
-        }
-        if (!whole) {  // a hidden key's scale may be NaN
-#pragma unroll
-          for (int k = 0; k < 4; k++)
-            if (!(seen >> (4 * c + k) & 1)) w[k] = 0.f;
-        }
+        const ulonglong2 v4 = vp[c];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-          const __half2 h = __floats2half2_rn(w[2 * k], w[2 * k + 1]);
+          float e0, e1;
+          unpack2(fma2(x[2 * c + k], rf2, mr2), e0, e1);
+          const f32x2 p = pack2(ex2(e0), ex2(e1));
+          sum[k] = add2(sum[k], p);
+          float w0, w1;
+          unpack2(mul2(p, k ? v4.y : v4.x), w0, w1);
+          const __half2 h = __floats2half2_rn(w0, w1);
           ph[2 * c + k] = h2_as_u32(h);
           if (SPLIT) {
             const float2 g = __half22float2(h);
-            pl[SPLIT ? 2 * c + k : 0] = h2_as_u32(__floats2half2_rn(w[2 * k] - g.x, w[2 * k + 1] - g.y));
+            pl[SPLIT ? 2 * c + k : 0] = h2_as_u32(__floats2half2_rn(w0 - g.x, w1 - g.y));
           }
         }
       }
-      l += sum;
+      if (vnan_s[sl] && !whole) {
+        // A key that this row does not see has a NaN scale: its weight is nothing.
+        const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
+#pragma unroll
+        for (int c = 0; c < FL_TILE / 2; c++) {
+          const uint32_t w = c < 16 ? s0 : s1;
+          const uint32_t keep = (w >> (2 * c & 31) & 1 ? 0xffffu : 0u) | (w >> (2 * c + 1 & 31) & 1 ? 0xffff0000u : 0u);
+          ph[c] &= keep;
+          if (SPLIT) pl[SPLIT ? c : 0] &= keep;
+        }
+      }
+      {
+        float a0, a1, b0, b1;
+        unpack2(sum[0], a0, a1);
+        unpack2(sum[1], b0, b1);
+        l += (a0 + a1) + (b0 + b1);
+      }
       tmem_st32(ts, ph);
       if constexpr (SPLIT) tmem_st32(ts + 32u, pl);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(p_full + (t & 1));  // two: a warp may be a tile ahead of another (S_{t+1} is there early)
     }
-    if (ok && ntile > 0) ok = warp_wait_or_abort(all_done, 0u, abort_flag, a.err);
+    if (ok && ntile > 0) ok = warp_wait_phase(all_done, 0u, abort_flag, a.err);
     tc_fence_after();
     // O (in the values' own scale), m and l to shared memory: Q, K and V are no
     // longer read (the last products have completed).
@@ -608,7 +726,7 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   int cl = 1;
   while (cl < 8 && ctas * cl * 2 <= 2 * device_sm_count() && a.CAP > 2 * FL_TILE * cl) cl *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * cl), (unsigned)a.KVH, (unsigned)a.B);
+  cfg.gridDim = dim3((unsigned)(a.KVH * cl), (unsigned)a.B, (unsigned)tiles);
   cfg.blockDim = dim3(FL_THREADS);
   cfg.dynamicSmemBytes = L::BYTES;
   cfg.stream = s;
@@ -636,7 +754,7 @@ void launch_out(const Kv8Args &a, cudaStream_t s) {
 bool kv8_flash_shape(const Kv8Args &a) {
   auto al = [](const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   const int64_t rows = (int64_t)a.S * (a.H / a.KVH);
-  return (a.D == 64 || a.D == 128) && rows > 48 && rows < (1 << 30) && a.KVH <= 65535 && a.q_rs % 4 == 0 &&
+  return (a.D == 64 || a.D == 128) && rows > 48 && rows <= 65535 * FL_ROWS && a.KVH <= 65535 && a.q_rs % 4 == 0 &&
          al(a.q, 16) && al(a.kc, 16) && al(a.vc, 16) && al(a.out, 16) && al(a.out16, 8) && al(a.q_gain, 16) &&
          (!a.cos || (a.rot % 8 == 0 && a.half % 4 == 0 && al(a.cos, 16) && al(a.sin, 16)));
 }

@@ -148,6 +148,251 @@ __device__ __forceinline__ void append_row(const Kv8Args &a, int b, int i, int k
                (side ? a.vc : a.kc) + row * a.D, (side ? a.vs : a.ks) + row, lane);
 }
 
+// ---- the same row with little double arithmetic ----------------------------
+// Rows of whole float4s (D % 4 == 0, aligned, rotary pairs in whole float4s): x is
+// formed in fp32, and only what that cannot decide goes through double: the
+// row's norm factor, the elements that may be the maximum, and an element whose
+// fp32 quotient lies within its error of a rounding border. Same codes and
+// scales as quantise_row.
+struct RowChunk {
+  float x[4], w[4];    // values and their rotary partners
+  float g[4], gw[4];   // head norm gains of both
+  float c[4], sn[4];   // x_rot = x c - w sn (the sign of the second half is in sn)
+};
+
+template <bool NORM, bool ROT>
+__device__ __forceinline__ double chunk_exact(const RowChunk &r, int k, double inv, bool turn) {
+  const double x = NORM ? (double)r.x[k] * inv * r.g[k] : (double)r.x[k];
+  if (!ROT || !turn) return x;
+  const double w = NORM ? (double)r.w[k] * inv * r.gw[k] : (double)r.w[k];
+  return x * (double)r.c[k] - w * (double)r.sn[k];
+}
+
+__device__ __forceinline__ uint32_t exact_code(double x, float s, bool e4m3) {
+  const double top = e4m3 ? 448.0 : 127.0, t = fmin(fmax(x / (double)s, -top), top);
+  return e4m3 ? e4m3_code(t) : (uint32_t)(uint8_t)(int8_t)(int)rint(t);
+}
+
+// NCH chunks of four values per lane: values 4 (lane + 32 i) .. + 3 of the row.
+// NORM: the head norm comes first; ROT: the chunks that `turn` marks are rotated.
+template <bool E4M3, int NCH, bool NORM, bool ROT>
+__device__ __forceinline__ void quantise_chunks(RowChunk (&r)[NCH], int D, double eps, const bool (&turn)[NCH],
+                                                uint8_t *codes, float *scale, int lane) {
+  constexpr bool real = NORM || ROT;  // x is more than its fp32 value
+  constexpr float top = E4M3 ? 448.f : 127.f;
+  double inv = 1.0;
+  float invf = 1.f;
+  if (NORM) {
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < NCH; i++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) ss = fma((double)r[i].x[k], (double)r[i].x[k], ss);
+    const double v = warp_sum_d(ss) / D + eps;
+    // 1 / sqrt(v): two Newton steps from the fp32 value (relative error 2^-50);
+    // outside fp32's comfortable range by the library
+    if (v > 1e-30 && v < 1e30) {
+      double y = rsqrtf((float)v);
+      y = y * fma(-0.5 * v * y, y, 1.5);
+      inv = y * fma(-0.5 * v * y, y, 1.5);
+    } else {
+      inv = 1.0 / sqrt(v);
+    }
+    invf = (float)inv;
+  }
+  float x[NCH][4];
+  uint32_t mx = 0;
+  float mag = 0.f;  // largest sum of the magnitudes that make up a value
+#pragma unroll
+  for (int i = 0; i < NCH; i++) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      float v = NORM ? r[i].x[k] * invf * r[i].g[k] : r[i].x[k];
+      if (ROT && turn[i]) {
+        const float w = NORM ? r[i].w[k] * invf * r[i].gw[k] : r[i].w[k];
+        const float p = v * r[i].c[k], q = w * r[i].sn[k];
+        v = p - q;
+        mag = fmaxf(mag, fabsf(p) + fabsf(q));
+      } else if (real) {
+        mag = fmaxf(mag, fabsf(v));
+      }
+      x[i][k] = v;
+      mx = max(mx, __float_as_uint(v) & 0x7fffffffu);  // infinities and NaN order above
+    }
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  const float amaxf = __uint_as_float(mx);
+  // |fp32 x - x|: at most seven roundings of 2^-24 of mag
+  const float xerr = real ? __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mag))) * 0x1p-20f : 0.f;
+  float s;
+  if (mx >= 0x7f800000u) {
+    s = __int_as_float(0x7fc00000);
+    // (an infinity that only the fp32 arithmetic made is told apart below)
+  } else if (!real) {
+    // amaxf / top, rounded once: Markstein's quotient by the rounded reciprocal
+    const float q = amaxf * (1.f / top);
+    s = fmaf(fmaf(-q, top, amaxf), 1.f / top, q);
+  } else {
+    double am = 0.0;
+    const float near = amaxf - 2.f * xerr;
+#pragma unroll
+    for (int i = 0; i < NCH; i++)
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (fabsf(x[i][k]) >= near) am = fmax(am, fabs(chunk_exact<NORM, ROT>(r[i], k, inv, turn[i])));
+    const unsigned cand = __ballot_sync(0xffffffffu, am > 0.0);  // one lane as a rule
+    am = (cand & (cand - 1)) == 0 ? __shfl_sync(0xffffffffu, am, cand ? __ffs(cand) - 1 : 0) : warp_max_d(am);
+    s = (float)(am * (1.0 / (double)top));
+  }
+  // Values near the ends of fp32's range: everything in double.
+  const bool slow_row = real ? !(amaxf > 1e-25f && amaxf < 1e30f) : !(amaxf > 1e-30f && mx < 0x7f800000u);
+  uint32_t word[NCH];
+  if (slow_row) {
+    double am = 0.0;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NCH; i++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const double v = chunk_exact<NORM, ROT>(r[i], k, inv, turn[i]);
+        bad |= !isfinite(v);
+        am = fmax(am, fabs(v));
+      }
+    bad = __any_sync(0xffffffffu, bad);
+    s = bad ? __int_as_float(0x7fc00000) : (float)(warp_max_d(am) / (double)top);
+#pragma unroll
+    for (int i = 0; i < NCH; i++) {
+      word[i] = 0;
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (s > 0.f) word[i] |= exact_code(chunk_exact<NORM, ROT>(r[i], k, inv, turn[i]), s, E4M3) << (8 * k);
+    }
+  } else {
+    const float is = __fdividef(1.f, s);  // (its error of some 2^-23 is within the 2^-20 below)
+    const float wabs = xerr * is;  // |t - x / s| is at most this and 2^-20 of t
+    uint32_t doubt = 0;
+#pragma unroll
+    for (int i = 0; i < NCH; i++) {
+      uint32_t c[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float t = x[i][k] * is, w = fmaf(fabsf(t), 0x1p-20f, wabs);
+        if (E4M3) {
+          const uint32_t p = __nv_cvt_float2_to_fp8x2(make_float2(t - w, t + w), __NV_SATFINITE, __NV_E4M3);
+          c[k] = p;
+          doubt |= ((p ^ (p >> 8)) & 0xffu) ? 1u << (4 * i + k) : 0u;
+        } else {
+          const uint32_t lo = __float_as_uint((t - w) + 12582912.f), hi = __float_as_uint((t + w) + 12582912.f);
+          c[k] = lo;
+          doubt |= lo != hi ? 1u << (4 * i + k) : 0u;
+        }
+      }
+      word[i] = b2m::prmt(b2m::prmt(c[0], c[1], 0x0040), b2m::prmt(c[2], c[3], 0x0040), 0x5410);
+    }
+    if (doubt) {
+#pragma unroll
+      for (int i = 0; i < NCH; i++)
+#pragma unroll 1
+        for (int k = 0; k < 4; k++) {
+          if (!(doubt >> (4 * i + k) & 1)) continue;
+          RowChunk e;  // (selected by hand: k is not a constant here)
+#pragma unroll
+          for (int u = 0; u < 4; u++)
+            if (u == k) {
+              e.x[0] = r[i].x[u], e.w[0] = r[i].w[u], e.g[0] = r[i].g[u];
+              e.gw[0] = r[i].gw[u], e.c[0] = r[i].c[u], e.sn[0] = r[i].sn[u];
+            }
+          const uint32_t code = exact_code(chunk_exact<NORM, ROT>(e, 0, inv, turn[i]), s, E4M3);
+          word[i] = (word[i] & ~(0xffu << (8 * k))) | (code << (8 * k));
+        }
+    }
+  }
+  if (lane == 0) *scale = s;
+#pragma unroll
+  for (int i = 0; i < NCH; i++)
+    if (4 * (lane + 32 * i) < D) *reinterpret_cast<uint32_t *>(codes + 4 * (lane + 32 * i)) = word[i];
+}
+
+// The rows quantise_chunks takes.
+inline bool append_rows_vec(const Kv8Args &a) {
+  auto al = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  return a.D % 4 == 0 && a.kv_rs % 4 == 0 && al(a.k) && al(a.v) && al(a.k_gain) &&
+         (!a.cos || (a.rot % 8 == 0 && a.half % 4 == 0 && al(a.cos) && al(a.sin)));
+}
+
+// Loads one side's row of new token i (position pos for the rotary).
+template <int NCH>
+__device__ __forceinline__ void load_chunks(const Kv8Args &a, const float *src, const float *gain, const float *cos,
+                                            int64_t pos, RowChunk (&r)[NCH], bool (&turn)[NCH], int lane) {
+#pragma unroll
+  for (int i = 0; i < NCH; i++) {
+    const int d = 4 * (lane + 32 * i);
+    turn[i] = false;
+    auto put = [](float *dst, const float *p) {
+      const float4 v = *reinterpret_cast<const float4 *>(p);
+      dst[0] = v.x, dst[1] = v.y, dst[2] = v.z, dst[3] = v.w;
+    };
+#pragma unroll
+    for (int k = 0; k < 4; k++) r[i].x[k] = r[i].w[k] = r[i].g[k] = r[i].gw[k] = r[i].c[k] = r[i].sn[k] = 0.f;
+    if (d >= a.D) continue;
+    put(r[i].x, src + d);
+    if (gain) put(r[i].g, gain + d);
+    if (cos && d < a.rot) {
+      turn[i] = true;
+      if (a.interleaved) {
+        const float2 c2 = *reinterpret_cast<const float2 *>(cos + pos * a.half + (d >> 1));
+        const float2 s2 = *reinterpret_cast<const float2 *>(a.sin + pos * a.half + (d >> 1));
+        r[i].c[0] = r[i].c[1] = c2.x, r[i].c[2] = r[i].c[3] = c2.y;
+        r[i].sn[0] = s2.x, r[i].sn[1] = -s2.x, r[i].sn[2] = s2.y, r[i].sn[3] = -s2.y;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          r[i].w[k] = r[i].x[k ^ 1];
+          r[i].gw[k] = r[i].g[k ^ 1];
+        }
+      } else {
+        const int hr = a.rot >> 1;
+        const bool first = d < hr;
+        const int pi = first ? d : d - hr, e = first ? d + hr : d - hr;
+        put(r[i].c, cos + pos * a.half + pi);
+        put(r[i].sn, a.sin + pos * a.half + pi);
+        put(r[i].w, src + e);
+        if (gain) put(r[i].gw, gain + e);
+        if (!first)
+#pragma unroll
+          for (int k = 0; k < 4; k++) r[i].sn[k] = -r[i].sn[k];
+      }
+    }
+  }
+}
+
+// append_row for rows that append_rows_vec accepts: both sides of new token i.
+template <bool E4M3, int NCH>
+__device__ __forceinline__ void append_pair_vec(const Kv8Args &a, int b, int i, int kvh, int past, int lane) {
+  const int64_t pos = token_pos(a, b, i, past);
+  if (past < 0 || (a.cos && pos < 0)) {
+    if (lane == 0 && a.err) b2m::set_dev_error(a.err, B2M_DEVERR_INDEX);
+    return;
+  }
+  if ((int64_t)past + i >= a.CAP) {
+    if (lane == 0 && a.err) b2m::set_dev_error(a.err, B2M_DEVERR_CACHE_FULL);
+    return;
+  }
+  const int64_t off = ((int64_t)b * a.S + i) * a.kv_rs + (int64_t)kvh * a.D;
+  const int64_t row = ((int64_t)b * a.KVH + kvh) * a.CAP + past + i;
+  const float *gain = a.k_gain ? a.k_gain + (int64_t)kvh * a.D : nullptr;
+  RowChunk rk[NCH], rv[NCH];
+  bool tk[NCH], tv[NCH];
+  load_chunks<NCH>(a, a.v + off, nullptr, nullptr, 0, rv, tv, lane);
+  load_chunks<NCH>(a, a.k + off, gain, pos >= a.CAP ? nullptr : a.cos, pos, rk, tk, lane);
+  quantise_chunks<E4M3, NCH, false, false>(rv, a.D, 0.0, tv, a.vc + row * a.D, a.vs + row, lane);
+  if (gain)  // (ROT without a table: no chunk is marked)
+    quantise_chunks<E4M3, NCH, true, true>(rk, a.D, a.eps, tk, a.kc + row * a.D, a.ks + row, lane);
+  else if (a.cos)
+    quantise_chunks<E4M3, NCH, false, true>(rk, a.D, 0.0, tk, a.kc + row * a.D, a.ks + row, lane);
+  else
+    quantise_chunks<E4M3, NCH, false, false>(rk, a.D, 0.0, tk, a.kc + row * a.D, a.ks + row, lane);
+}
+
 // Two e-th codes of words a and b interleaved: prmt selectors for codes 0, 1
 // and codes 2, 3 of both.
 constexpr uint32_t PAIR01 = 0x5140, PAIR23 = 0x7362;
