@@ -204,102 +204,30 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   }
   if (warp == 8) tmem_alloc(slot, 256);
 
-  // Q rows, eight lanes each (lane l8 holds the float4 chunks l8 + 8 i): head
-  // norm, rotary, scaled by a power of two to a largest magnitude in [2^9, 2^10).
-  {
-    constexpr int NC = D / 32;  // chunks per lane
-    const int l8 = lane & 7;
-    for (int rr = warp * 4 + (lane >> 3); rr < FL_ROWS; rr += FL_THREADS / 8) {
-      const int r = row0 + rr;
-      const bool valid = r < nrows;
-      const int i = valid ? r / G : 0, h = kvh * G + (valid ? r % G : 0);
-      const float *src = a.q + ((int64_t)b * a.S + i) * a.q_rs + (int64_t)h * D;
-      const float *gain = a.q_gain ? a.q_gain + (int64_t)h * D : nullptr;
-      const int64_t pos = token_pos(a, b, i, past);
-      const bool turn = a.cos && pos >= 0 && pos < a.CAP;
-      const int hr = a.rot >> 1;
-      float4 v[NC];
+  for (int rr = warp * 4 + (lane >> 3); rr < FL_ROWS; rr += FL_THREADS / 8) {
+    QRow<D> q;
+    load_q_row<D>(a, b, kvh, G, row0 + rr, past, code_factor<E4M3>(), q);
 #pragma unroll
-      for (int u = 0; u < NC; u++) v[u] = *reinterpret_cast<const float4 *>(src + 4 * (l8 + 8 * u));
-      float inv = 1.f;
-      if (gain) {
-        float ss = 0.f;
-#pragma unroll
-        for (int u = 0; u < NC; u++)
-          ss = fmaf(v[u].x, v[u].x, fmaf(v[u].y, v[u].y, fmaf(v[u].z, v[u].z, fmaf(v[u].w, v[u].w, ss))));
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        inv = 1.f / sqrtf(ss / D + (float)a.eps);
-      }
-      float mx = 0.f;
-#pragma unroll
-      for (int u = 0; u < NC; u++) {
-        const int d = 4 * (l8 + 8 * u);
-        float x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-        if (gain) {
-          const float4 g4 = *reinterpret_cast<const float4 *>(gain + d);
-          x[0] *= inv * g4.x, x[1] *= inv * g4.y, x[2] *= inv * g4.z, x[3] *= inv * g4.w;
-        }
-        if (turn && d < a.rot) {
-          // (the launcher takes rotary_dim % 8 == 0: a chunk and its partner are whole float4s)
-          const bool first = a.interleaved || d < hr;
-          float c[4], sn[4], w[4];
-          if (a.interleaved) {
-            const float2 c2 = *reinterpret_cast<const float2 *>(a.cos + pos * a.half + (d >> 1));
-            const float2 s2 = *reinterpret_cast<const float2 *>(a.sin + pos * a.half + (d >> 1));
-            c[0] = c[1] = c2.x, c[2] = c[3] = c2.y;
-            sn[0] = s2.x, sn[1] = -s2.x, sn[2] = s2.y, sn[3] = -s2.y;
-            w[0] = x[1], w[1] = x[0], w[2] = x[3], w[3] = x[2];
-          } else {
-            const int pi = first ? d : d - hr, e = first ? d + hr : d - hr;
-            const float4 c4 = *reinterpret_cast<const float4 *>(a.cos + pos * a.half + pi);
-            const float4 s4 = *reinterpret_cast<const float4 *>(a.sin + pos * a.half + pi);
-            float4 w4 = *reinterpret_cast<const float4 *>(src + e);
-            if (gain) {
-              const float4 g4 = *reinterpret_cast<const float4 *>(gain + e);
-              w4.x *= inv * g4.x, w4.y *= inv * g4.y, w4.z *= inv * g4.z, w4.w *= inv * g4.w;
-            }
-            c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w;
-            const float sg = first ? 1.f : -1.f;
-            sn[0] = sg * s4.x, sn[1] = sg * s4.y, sn[2] = sg * s4.z, sn[3] = sg * s4.w;
-            w[0] = w4.x, w[1] = w4.y, w[2] = w4.z, w[3] = w4.w;
-          }
-#pragma unroll
-          for (int k = 0; k < 4; k++) x[k] = x[k] * c[k] - w[k] * sn[k];
-        }
-        v[u] = valid ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      // mx = f 2^e, f in [1/2, 1), times 2^(10 - e) in two steps (either may leave
-      // the normal range alone). Zero, infinite and NaN rows: any exponent does.
-      int e = 10;
-      if (mx > 0.f && mx < INFINITY) frexpf(mx, &e);
-      const int e1 = (10 - e) / 2, e2 = 10 - e - e1;
-      const float f1 = __uint_as_float((uint32_t)(127 + e1) << 23), f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
-#pragma unroll
-      for (int u = 0; u < NC; u++) {
-        const int d = 4 * (l8 + 8 * u);
-        const float4 x = make_float4(v[u].x * f1 * f2, v[u].y * f1 * f2, v[u].z * f1 * f2, v[u].w * f1 * f2);
-        const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
-        const uint32_t at = (uint32_t)(d >> 6) * 16384u + sw128(rr, d & 63);
-        *reinterpret_cast<uint2 *>(smem + L::QH + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
-        if (SPLIT) {
-          const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
-          *reinterpret_cast<uint2 *>(smem + L::QL + at) =
-              make_uint2(h2_as_u32(__floats2half2_rn(x.x - g0.x, x.y - g0.y)),
-                         h2_as_u32(__floats2half2_rn(x.z - g1.x, x.w - g1.y)));
-        }
-      }
-      if (l8 == 0) {
-        row_factor[rr] = ldexpf(a.scale * LOG2E * code_factor<E4M3>(), e - 10);
-        row_lim[rr] = !valid ? -1 : (a.tree ? past - 1 : past + i);
-        row_bits[rr] = valid && a.tree ? a.tree[(int64_t)b * a.S + i] : 0;
+    for (int u = 0; u < D / 32; u++) {
+      const int d = 4 * ((lane & 7) + 8 * u);
+      const float4 x = q.v[u];
+      const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
+      const uint32_t at = (uint32_t)(d >> 6) * 16384u + sw128(rr, d & 63);
+      *reinterpret_cast<uint2 *>(smem + L::QH + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
+      if (SPLIT) {
+        const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
+        *reinterpret_cast<uint2 *>(smem + L::QL + at) =
+            make_uint2(h2_as_u32(__floats2half2_rn(x.x - g0.x, x.y - g0.y)),
+                       h2_as_u32(__floats2half2_rn(x.z - g1.x, x.w - g1.y)));
       }
     }
-    fence_proxy_async_smem();
+    if ((lane & 7) == 0) {
+      row_factor[rr] = q.factor;
+      row_lim[rr] = q.lim;
+      row_bits[rr] = q.bits;
+    }
   }
+  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -749,14 +677,13 @@ void launch_out(const Kv8Args &a, cudaStream_t s) {
 
 }  // namespace
 
-// Enough rows to fill most of a 128-row tile; head dims, alignments and rotary
-// widths whose float4 chunks the prologue can take.
+// Enough rows to fill most of a 128-row tile, head dims and alignments the
+// kernel takes.
 bool kv8_flash_shape(const Kv8Args &a) {
   auto al = [](const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   const int64_t rows = (int64_t)a.S * (a.H / a.KVH);
-  return (a.D == 64 || a.D == 128) && rows > 48 && rows <= 65535 * FL_ROWS && a.KVH <= 65535 && a.q_rs % 4 == 0 &&
-         al(a.q, 16) && al(a.kc, 16) && al(a.vc, 16) && al(a.out, 16) && al(a.out16, 8) && al(a.q_gain, 16) &&
-         (!a.cos || (a.rot % 8 == 0 && a.half % 4 == 0 && al(a.cos, 16) && al(a.sin, 16)));
+  return (a.D == 64 || a.D == 128) && rows > 48 && rows <= 65535 * FL_ROWS && a.KVH <= 65535 && q_rows_vec(a) &&
+         al(a.kc, 16) && al(a.vc, 16) && al(a.out, 16) && al(a.out16, 8);
 }
 
 // The call's keys and values must have been appended.

@@ -78,10 +78,8 @@ struct StepSmem {
   static constexpr int ROWS = QF + NT * StepShape<D>::KSTEPS * 512;            // per-row words, below
   // bits[R] (u64), factor[R], lim[R], wm[4][R], wl[4][R], cm[R], cl[R]
   static constexpr int BYTES = ROWS + R * (8 + 4 + 4 + 16 + 16 + 8);
-  // Warp states O [4][R][D] fp32, and the prologue's staging rows, reuse the
-  // ring (drained by then / not yet filled).
+  // Warp states O [4][R][D] fp32 reuse the ring (drained by then).
   static_assert(ST_WARPS * R * D * 4 <= QF, "O staging fits the ring");
-  static_assert((R + ST_WARPS) * 256 * 4 <= QF || (R * D + ST_WARPS * 256) * 4 <= QF, "Q staging fits the ring");
 };
 
 template <bool E4M3, int D, int NT>
@@ -111,92 +109,6 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
   const int chunk = (((n + CL - 1) / CL) + 15) & ~15;
   const int jbeg = min(n, rank * chunk), jend = min(n, jbeg + chunk);
   const int64_t base = ((int64_t)b * a.KVH + kvh) * a.CAP;
-
-  // New rows that fall into this CTA's range (every rank sees to its own, the
-  // last one also reports those past the capacity).
-  if (fused_append) {
-    float *stage = reinterpret_cast<float *>(smem) + warp * 256;
-    const int i0 = max(0, jbeg - past), i1 = rank == CL - 1 ? a.S : min(a.S, jend - past);
-    for (int it = 2 * i0 + warp; it < 2 * i1; it += ST_WARPS)
-      if (past + (it >> 1) >= jbeg) append_row(a, b, it >> 1, kvh, it & 1, a.past[b], stage, lane);
-    __syncthreads();
-  }
-
-  // Q rows: head norm, rotary, scaled to a largest magnitude in [2^9, 2^10) by a
-  // power of two that joins the row's factor.
-  {
-    float *qs = reinterpret_cast<float *>(smem) + ST_WARPS * 256;
-    for (int rr = warp; rr < R; rr += ST_WARPS) {
-      const int r = row0 + rr;
-      float *x = qs + rr * D;
-      const bool valid = r < nrows;
-      const int i = valid ? r / G : 0, h = kvh * G + (valid ? r % G : 0);
-      const float *src = a.q + ((int64_t)b * a.S + i) * a.q_rs + (int64_t)h * D;
-      float v[D / 32];
-      float ss = 0.f;
-#pragma unroll
-      for (int u = 0; u < D / 32; u++) {
-        v[u] = valid ? src[lane + 32 * u] : 0.f;
-        ss = fmaf(v[u], v[u], ss);
-      }
-      if (a.q_gain) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = (float)(1.0 / sqrt((double)ss / D + a.eps));
-#pragma unroll
-        for (int u = 0; u < D / 32; u++) v[u] = valid ? v[u] * inv * a.q_gain[(int64_t)h * D + lane + 32 * u] : 0.f;
-      }
-      if (a.cos) {
-#pragma unroll
-        for (int u = 0; u < D / 32; u++) x[lane + 32 * u] = v[u];
-        __syncwarp();
-        const int64_t pos = token_pos(a, b, i, past);
-        if (valid && pos >= 0 && pos < a.CAP) {
-          const int hr = a.rot >> 1;
-#pragma unroll
-          for (int u = 0; u < D / 32; u++) {
-            const int d = lane + 32 * u;
-            if (d >= a.rot) continue;
-            const bool first = a.interleaved ? (d & 1) == 0 : d < hr;
-            const int pi = a.interleaved ? d >> 1 : (first ? d : d - hr);
-            const int e = a.interleaved ? (d ^ 1) : (first ? d + hr : d - hr);
-            const float c = a.cos[pos * a.half + pi], sn = a.sin[pos * a.half + pi], w = x[e];
-            v[u] = first ? v[u] * c - w * sn : v[u] * c + w * sn;
-          }
-        }
-        __syncwarp();
-      }
-      float mx = 0.f;
-#pragma unroll
-      for (int u = 0; u < D / 32; u++) mx = fmaxf(mx, fabsf(v[u]));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      // mx = f 2^e with f in [1/2, 1): scaled by 2^(10 - e). Zero, infinite and
-      // (ignored by fmaxf) NaN rows: any exponent does.
-      int e = 10;
-      if (mx > 0.f && mx < INFINITY) frexpf(mx, &e);
-#pragma unroll
-      for (int u = 0; u < D / 32; u++) x[lane + 32 * u] = ldexpf(v[u], 10 - e);
-      if (lane == 0) {
-        row_factor[rr] = ldexpf(a.scale * LOG2E * code_factor<E4M3>(), e - 10);
-        row_lim[rr] = !valid ? -1 : (a.tree ? past - 1 : past + i);
-        row_bits[rr] = valid && a.tree ? a.tree[(int64_t)b * a.S + i] : 0;
-      }
-    }
-    __syncthreads();
-    // Fragments: element pairs of a k-step in the order the codes' words give.
-    for (int e = tid; e < NT * L::KSTEPS * 32; e += ST_THREADS) {
-      const int ln = e & 31, ks = (e >> 5) % L::KSTEPS, nt = (e >> 5) / L::KSTEPS;
-      const int d = ((ks / L::KW) * 4 + (ln & 3)) * L::KC + 4 * (ks % L::KW);
-      const float4 x = *reinterpret_cast<const float4 *>(qs + (nt * 8 + (ln >> 2)) * D + d);
-      const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
-      const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-      qfrag[e] = make_uint4(b2m::h2_as_u32(h0), b2m::h2_as_u32(h1),
-                            b2m::h2_as_u32(__floats2half2_rn(x.x - f0.x, x.y - f0.y)),
-                            b2m::h2_as_u32(__floats2half2_rn(x.z - f1.x, x.w - f1.y)));
-    }
-    __syncthreads();
-  }
 
   // Ring of this warp.
   uint8_t *ring = smem + warp * (ST_STAGES * L::SLOT);
@@ -228,6 +140,55 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
     cp_commit();
   };
 
+  // The first tiles are on their way while the rows below are prepared (a tile
+  // with rows that this call still appends waits for them).
+  int ahead = 0;
+#pragma unroll
+  for (int k = 0; k < ST_STAGES - 1; k++)
+    if (ahead == k && (!fused_append || jbeg + 16 * (warp + k * ST_WARPS) + 16 <= past)) {
+      issue(warp + k * ST_WARPS, k);
+      ahead = k + 1;
+    }
+  // Work items of the prologue, dealt to the warps: the new rows of this CTA's
+  // range (every rank appends its own, the last one also reports those past the
+  // capacity), then groups of four query rows.
+  {
+    const int i0 = max(0, jbeg - past), i1 = !fused_append ? i0 : (rank == CL - 1 ? a.S : min(a.S, jend - past));
+    const int nnew = 2 * max(0, i1 - i0);
+    for (int it = warp; it < nnew + R / 4; it += ST_WARPS) {
+      if (it < nnew) {
+        append_side_vec<E4M3, (D + 127) / 128>(a, b, i0 + (it >> 1), kvh, it & 1, a.past[b], lane);
+      } else {
+        const int rr = 4 * (it - nnew) + (lane >> 3);
+        QRow<D> q;
+        load_q_row<D>(a, b, kvh, G, row0 + rr, past, code_factor<E4M3>(), q);
+#pragma unroll
+        for (int u = 0; u < D / 32; u++) {
+          // Fragment of values d .. d + 3: the k-step, and the lane of the row's
+          // four, whose code words hold them.
+          const int d = 4 * ((lane & 7) + 8 * u);
+          const int ks = d / (4 * L::KC) * L::KW + d % L::KC / 4, t4 = d / L::KC % 4;
+          const float4 x = q.v[u];
+          const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
+          const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+          qfrag[((rr >> 3) * L::KSTEPS + ks) * 32 + (rr & 7) * 4 + t4] =
+              make_uint4(b2m::h2_as_u32(h0), b2m::h2_as_u32(h1),
+                         b2m::h2_as_u32(__floats2half2_rn(x.x - f0.x, x.y - f0.y)),
+                         b2m::h2_as_u32(__floats2half2_rn(x.z - f1.x, x.w - f1.y)));
+        }
+        if ((lane & 7) == 0) {
+          row_factor[rr] = q.factor;
+          row_lim[rr] = q.lim;
+          row_bits[rr] = q.bits;
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ST_STAGES - 1; k++)
+      if (k >= ahead) issue(warp + k * ST_WARPS, k);
+  }
+
   float o[NT][L::MT][4];
   float m[NT][2], mref[NT][2], l[NT][2], rf[NT][2];
 #pragma unroll
@@ -247,8 +208,6 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
   float vmax = 0.f, vinv = 0.f;  // largest V scale seen (a power of two above it), and its reciprocal
   const int all_see = a.tree ? past : past + row0 / G + 1;  // keys below this are seen by every row
 
-#pragma unroll
-  for (int s = 0; s < ST_STAGES - 1; s++) issue(warp + s * ST_WARPS, s);
   int slot = 0;
   for (int tile = warp; tile < ntile; tile += ST_WARPS) {
     cp_wait<ST_STAGES - 2>();
@@ -257,11 +216,11 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
     const uint8_t *s = ring + slot * L::SLOT;
     const int j0 = jbeg + 16 * tile;
     // S^T = K . Q^T
-    float c[NT][4];
+    float c[NT][4], cl[NT][4];  // (two chains of products: half the latency)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int u = 0; u < 4; u++) c[nt][u] = 0.f;
+      for (int u = 0; u < 4; u++) c[nt][u] = cl[nt][u] = 0.f;
 #pragma unroll
     for (int cc = 0; cc < L::NKC; cc++) {
       uint32_t w0[L::KW], w1[L::KW];
@@ -284,7 +243,7 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
         for (int nt = 0; nt < NT; nt++) {
           const uint4 q = qfrag[(nt * L::KSTEPS + cc * L::KW + w) * 32 + lane];
           b2m::mma_16816(c[nt], A, q.x, q.y, c[nt]);
-          b2m::mma_16816(c[nt], A, q.z, q.w, c[nt]);
+          b2m::mma_16816(cl[nt], A, q.z, q.w, cl[nt]);
         }
       }
     }
@@ -295,8 +254,8 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        x[nt][0][u] = c[nt][u] * sc.x * rf[nt][u];
-        x[nt][1][u] = c[nt][2 + u] * sc.y * rf[nt][u];
+        x[nt][0][u] = (c[nt][u] + cl[nt][u]) * sc.x * rf[nt][u];
+        x[nt][1][u] = (c[nt][2 + u] + cl[nt][2 + u]) * sc.y * rf[nt][u];
       }
     const bool whole = j0 + 16 <= min(jend, all_see);
     uint32_t seen = 0xffffffffu;  // bit (nt * 2 + key) * 2 + row
@@ -502,7 +461,8 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   constexpr auto kern = kv8_step_kernel<E4M3, D, NT>;
   b2m::set_smem_limit_once<kern>(M::BYTES);
   const int nrows = a.S * (a.H / a.KVH), tiles = (nrows + M::R - 1) / M::R;
-  if (tiles > 1) launch_kv8_append(a, s);
+  const bool fused = tiles == 1 && append_rows_vec(a);
+  if (!fused) launch_kv8_append(a, s);
   // Key splits: CTAs for four per SM, at least 64 cache positions each.
   const int64_t ctas = (int64_t)a.B * a.KVH * tiles;
   int cl = 1;
@@ -518,7 +478,7 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  B2M_CUDA(cudaLaunchKernelEx(&cfg, kern, a, tiles == 1 ? 1 : 0));
+  B2M_CUDA(cudaLaunchKernelEx(&cfg, kern, a, fused ? 1 : 0));
 }
 
 template <bool E4M3, int D>
@@ -543,11 +503,11 @@ void launch_dim(const Kv8Args &a, cudaStream_t s) {
 }  // namespace
 
 // Head dims the kernel is compiled for, cache rows it can copy 16 bytes at a
-// time, outputs it can store four values at a time.
+// time, query rows and outputs it can take four values at a time.
 bool kv8_step_shape(const Kv8Args &a) {
   auto al = [](const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
-  return (a.D == 32 || a.D == 64 || a.D == 96 || a.D == 128 || a.D == 256) && al(a.kc, 16) && al(a.vc, 16) &&
-         al(a.out, 16) && al(a.out16, 8) && a.KVH <= 65535;
+  return (a.D == 32 || a.D == 64 || a.D == 96 || a.D == 128 || a.D == 256) && q_rows_vec(a) && al(a.kc, 16) &&
+         al(a.vc, 16) && al(a.out, 16) && al(a.out16, 8) && a.KVH <= 65535;
 }
 
 void launch_kv8_step(const Kv8Args &a, cudaStream_t s) {

@@ -393,6 +393,135 @@ __device__ __forceinline__ void append_pair_vec(const Kv8Args &a, int b, int i, 
     quantise_chunks<E4M3, NCH, false, false>(rk, a.D, 0.0, tk, a.kc + row * a.D, a.ks + row, lane);
 }
 
+// One side of append_pair_vec.
+template <bool E4M3, int NCH>
+__device__ __forceinline__ void append_side_vec(const Kv8Args &a, int b, int i, int kvh, int side, int past, int lane) {
+  const int64_t pos = token_pos(a, b, i, past);
+  if (past < 0 || (a.cos && pos < 0)) {
+    if (lane == 0 && a.err) b2m::set_dev_error(a.err, B2M_DEVERR_INDEX);
+    return;
+  }
+  if ((int64_t)past + i >= a.CAP) {
+    if (lane == 0 && a.err) b2m::set_dev_error(a.err, B2M_DEVERR_CACHE_FULL);
+    return;
+  }
+  const int64_t off = ((int64_t)b * a.S + i) * a.kv_rs + (int64_t)kvh * a.D;
+  const int64_t row = ((int64_t)b * a.KVH + kvh) * a.CAP + past + i;
+  const float *gain = a.k_gain ? a.k_gain + (int64_t)kvh * a.D : nullptr;
+  const float *cos = pos >= a.CAP ? nullptr : a.cos;  // the table's positions
+  RowChunk r[NCH];
+  bool turn[NCH];
+  if (side) {
+    load_chunks<NCH>(a, a.v + off, nullptr, nullptr, 0, r, turn, lane);
+    quantise_chunks<E4M3, NCH, false, false>(r, a.D, 0.0, turn, a.vc + row * a.D, a.vs + row, lane);
+    return;
+  }
+  load_chunks<NCH>(a, a.k + off, gain, cos, pos, r, turn, lane);
+  if (gain)  // (ROT without a table: no chunk is marked)
+    quantise_chunks<E4M3, NCH, true, true>(r, a.D, a.eps, turn, a.kc + row * a.D, a.ks + row, lane);
+  else if (a.cos)
+    quantise_chunks<E4M3, NCH, false, true>(r, a.D, 0.0, turn, a.kc + row * a.D, a.ks + row, lane);
+  else
+    quantise_chunks<E4M3, NCH, false, false>(r, a.D, 0.0, turn, a.kc + row * a.D, a.ks + row, lane);
+}
+
+// ---- query rows -------------------------------------------------------------
+// Row r of a kv head's query rows is head r % G of token r / G. Eight lanes hold a
+// row (lane l8 the float4 chunks l8 + 8 i), four rows a warp: head norm, rotary,
+// and a power of two that brings its largest magnitude into [2^9, 2^10), where two
+// f16 terms hold 22 bits of it. All 32 lanes call it; rows past the last are zero.
+template <int D>
+struct QRow {
+  float4 v[D / 32];
+  float factor;   // what a score of these values is multiplied by (log2 units, K's scale apart)
+  int lim;        // last key seen whatever the tree says, -1: none
+  uint64_t bits;  // tree bits
+};
+
+// What the float4 loads below need.
+inline bool q_rows_vec(const Kv8Args &a) {
+  auto al = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  return a.D % 32 == 0 && a.q_rs % 4 == 0 && al(a.q) && al(a.q_gain) &&
+         (!a.cos || (a.rot % 8 == 0 && a.half % 4 == 0 && al(a.cos) && al(a.sin)));
+}
+
+template <int D>
+__device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int G, int r, int past, float code_scale,
+                                           QRow<D> &o) {
+  constexpr int NC = D / 32;
+  const int l8 = threadIdx.x & 7;
+  const bool valid = r < a.S * G;
+  const int i = valid ? r / G : 0, h = kvh * G + (valid ? r % G : 0);
+  const float *src = a.q + ((int64_t)b * a.S + i) * a.q_rs + (int64_t)h * D;
+  const float *gain = a.q_gain ? a.q_gain + (int64_t)h * D : nullptr;
+  const int64_t pos = token_pos(a, b, i, past);
+  const bool turn = a.cos && pos >= 0 && pos < a.CAP;
+  const int hr = a.rot >> 1;
+#pragma unroll
+  for (int u = 0; u < NC; u++) o.v[u] = *reinterpret_cast<const float4 *>(src + 4 * (l8 + 8 * u));
+  float inv = 1.f;
+  if (gain) {
+    float ss = 0.f;
+#pragma unroll
+    for (int u = 0; u < NC; u++)
+      ss = fmaf(o.v[u].x, o.v[u].x, fmaf(o.v[u].y, o.v[u].y, fmaf(o.v[u].z, o.v[u].z, fmaf(o.v[u].w, o.v[u].w, ss))));
+#pragma unroll
+    for (int f = 1; f < 8; f <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, f);
+    inv = 1.f / sqrtf(ss / D + (float)a.eps);
+  }
+  float mx = 0.f;
+#pragma unroll
+  for (int u = 0; u < NC; u++) {
+    const int d = 4 * (l8 + 8 * u);
+    float x[4] = {o.v[u].x, o.v[u].y, o.v[u].z, o.v[u].w};
+    if (gain) {
+      const float4 g4 = *reinterpret_cast<const float4 *>(gain + d);
+      x[0] *= inv * g4.x, x[1] *= inv * g4.y, x[2] *= inv * g4.z, x[3] *= inv * g4.w;
+    }
+    if (turn && d < a.rot) {
+      const bool first = a.interleaved || d < hr;
+      float c[4], sn[4], w[4];
+      if (a.interleaved) {
+        const float2 c2 = *reinterpret_cast<const float2 *>(a.cos + pos * a.half + (d >> 1));
+        const float2 s2 = *reinterpret_cast<const float2 *>(a.sin + pos * a.half + (d >> 1));
+        c[0] = c[1] = c2.x, c[2] = c[3] = c2.y;
+        sn[0] = s2.x, sn[1] = -s2.x, sn[2] = s2.y, sn[3] = -s2.y;
+        w[0] = x[1], w[1] = x[0], w[2] = x[3], w[3] = x[2];
+      } else {
+        const int pi = first ? d : d - hr, e = first ? d + hr : d - hr;
+        const float4 c4 = *reinterpret_cast<const float4 *>(a.cos + pos * a.half + pi);
+        const float4 s4 = *reinterpret_cast<const float4 *>(a.sin + pos * a.half + pi);
+        float4 w4 = *reinterpret_cast<const float4 *>(src + e);
+        if (gain) {
+          const float4 g4 = *reinterpret_cast<const float4 *>(gain + e);
+          w4.x *= inv * g4.x, w4.y *= inv * g4.y, w4.z *= inv * g4.z, w4.w *= inv * g4.w;
+        }
+        c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w;
+        const float sg = first ? 1.f : -1.f;
+        sn[0] = sg * s4.x, sn[1] = sg * s4.y, sn[2] = sg * s4.z, sn[3] = sg * s4.w;
+        w[0] = w4.x, w[1] = w4.y, w[2] = w4.z, w[3] = w4.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) x[k] = x[k] * c[k] - w[k] * sn[k];
+    }
+    o.v[u] = valid ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+  }
+#pragma unroll
+  for (int f = 1; f < 8; f <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, f));
+  // 2^(e-1) <= mx < 2^e (subnormals count as 2^-126, infinite rows as any), times
+  // 2^(10 - e) in two steps, as either may leave the normal range alone.
+  const int e = min(max((int)(__float_as_uint(mx) >> 23), 1), 254) - 126;
+  const int e1 = (10 - e) / 2, e2 = 10 - e - e1;
+  const float f1 = __uint_as_float((uint32_t)(127 + e1) << 23), f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
+#pragma unroll
+  for (int u = 0; u < NC; u++)
+    o.v[u] = make_float4(o.v[u].x * f1 * f2, o.v[u].y * f1 * f2, o.v[u].z * f1 * f2, o.v[u].w * f1 * f2);
+  o.factor = a.scale * LOG2E * code_scale / f1 / f2;
+  o.lim = !valid ? -1 : (a.tree ? past - 1 : past + i);
+  o.bits = valid && a.tree ? a.tree[(int64_t)b * a.S + i] : 0;
+}
+
 // Two e-th codes of words a and b interleaved: prmt selectors for codes 0, 1
 // and codes 2, 3 of both.
 constexpr uint32_t PAIR01 = 0x5140, PAIR23 = 0x7362;
