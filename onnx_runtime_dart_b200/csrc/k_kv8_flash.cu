@@ -206,11 +206,13 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
 
   for (int rr = warp * 4 + (lane >> 3); rr < FL_ROWS; rr += FL_THREADS / 8) {
     QRow<D> q;
-    load_q_row<D>(a, b, kvh, G, row0 + rr, past, code_factor<E4M3>(), q);
+    load_q_row<D>(a, b, kvh, G, row0 + rr, past, q);
 #pragma unroll
     for (int u = 0; u < D / 32; u++) {
       const int d = 4 * ((lane & 7) + 8 * u);
-      const float4 x = q.v[u];
+      // (in the order of K's expanded codes)
+      const float v[4] = {q.v[u].x, q.v[u].y, q.v[u].z, q.v[u].w};
+      const float4 x = make_float4(v[0], v[expand_order<E4M3>(1)], v[expand_order<E4M3>(2)], v[3]);
       const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
       const uint32_t at = (uint32_t)(d >> 6) * 16384u + sw128(rr, d & 63);
       *reinterpret_cast<uint2 *>(smem + L::QH + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
@@ -343,8 +345,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           uint32_t o[4];  // dims 4k .. 4k+3: keys (2p, 2p+1)
-          expand4<E4M3>(prmt(w0[k], w1[k], PAIR01), o[0], o[1]);
-          expand4<E4M3>(prmt(w0[k], w1[k], PAIR23), o[2], o[3]);
+          expand_zip<E4M3>(w0[k], w1[k], o);
 #pragma unroll
           for (int e = 0; e < 4; e++)
             *reinterpret_cast<uint32_t *>(vd + sw128(16 * (cw * VI + u) + 4 * k + e, 2 * lane)) = o[e];
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     // longer read (the last products have completed).
     float *ost = reinterpret_cast<float *>(smem) + rr * L::OST;
     if (ok) {
-      const float vo = ntile > 0 ? *vref_s * code_factor<E4M3>() : 0.f;
+      const float vo = ntile > 0 ? *vref_s : 0.f;
 #pragma unroll
       for (int c = 0; c < D / 16; c++) {
         uint32_t u[16];

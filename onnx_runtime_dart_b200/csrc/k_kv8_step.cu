@@ -161,14 +161,15 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
       } else {
         const int rr = 4 * (it - nnew) + (lane >> 3);
         QRow<D> q;
-        load_q_row<D>(a, b, kvh, G, row0 + rr, past, code_factor<E4M3>(), q);
+        load_q_row<D>(a, b, kvh, G, row0 + rr, past, q);
 #pragma unroll
         for (int u = 0; u < D / 32; u++) {
           // Fragment of values d .. d + 3: the k-step, and the lane of the row's
           // four, whose code words hold them.
           const int d = 4 * ((lane & 7) + 8 * u);
           const int ks = d / (4 * L::KC) * L::KW + d % L::KC / 4, t4 = d / L::KC % 4;
-          const float4 x = q.v[u];
+          const float v[4] = {q.v[u].x, q.v[u].y, q.v[u].z, q.v[u].w};
+          const float4 x = make_float4(v[0], v[expand_order<E4M3>(1)], v[expand_order<E4M3>(2)], v[3]);
           const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
           const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
           qfrag[((rr >> 3) * L::KSTEPS + ks) * 32 + (rr & 7) * 4 + t4] =
@@ -354,11 +355,10 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
       }
 #pragma unroll
       for (int w = 0; w < L::VW; w++) {
-        uint32_t A[2][4];  // dims 4w, 4w+1 and 4w+2, 4w+3 of the chunk
-        expand4<E4M3>(b2m::prmt(vw[0][w], vw[1][w], PAIR01), A[0][0], A[0][1]);
-        expand4<E4M3>(b2m::prmt(vw[2][w], vw[3][w], PAIR01), A[0][2], A[0][3]);
-        expand4<E4M3>(b2m::prmt(vw[0][w], vw[1][w], PAIR23), A[1][0], A[1][1]);
-        expand4<E4M3>(b2m::prmt(vw[2][w], vw[3][w], PAIR23), A[1][2], A[1][3]);
+        uint32_t lo[4], hi[4];  // dims 4w .. 4w+3 of the chunk: keys (2t, 2t+1), (2t+8, 2t+9)
+        expand_zip<E4M3>(vw[0][w], vw[1][w], lo);
+        expand_zip<E4M3>(vw[2][w], vw[3][w], hi);
+        const uint32_t A[2][4] = {{lo[0], lo[1], hi[0], hi[1]}, {lo[2], lo[3], hi[2], hi[3]}};
 #pragma unroll
         for (int hf = 0; hf < 2; hf++)
 #pragma unroll
@@ -377,7 +377,6 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
 
   // Warp states: m, l per row and O (in the values' own scale).
   float *so = reinterpret_cast<float *>(smem);
-  const float vs_out = vmax * code_factor<E4M3>();
 #pragma unroll
   for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -395,7 +394,7 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
       for (int k = 0; k < L::MT; k++) {
         const int cc = (k >> 1) / L::VW, w = (k >> 1) % L::VW;
         const int d = (cc * 8 + g) * L::VC + 4 * w + 2 * (k & 1);
-        *reinterpret_cast<float2 *>(dst + d) = make_float2(o[nt][k][u] * vs_out, o[nt][k][2 + u] * vs_out);
+        *reinterpret_cast<float2 *>(dst + d) = make_float2(o[nt][k][u] * vmax, o[nt][k][2 + u] * vmax);
       }
     }
   __syncthreads();

@@ -446,8 +446,7 @@ inline bool q_rows_vec(const Kv8Args &a) {
 }
 
 template <int D>
-__device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int G, int r, int past, float code_scale,
-                                           QRow<D> &o) {
+__device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int G, int r, int past, QRow<D> &o) {
   constexpr int NC = D / 32;
   const int l8 = threadIdx.x & 7;
   const bool valid = r < a.S * G;
@@ -517,35 +516,60 @@ __device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int
 #pragma unroll
   for (int u = 0; u < NC; u++)
     o.v[u] = make_float4(o.v[u].x * f1 * f2, o.v[u].y * f1 * f2, o.v[u].z * f1 * f2, o.v[u].w * f1 * f2);
-  o.factor = a.scale * LOG2E * code_scale / f1 / f2;
+  o.factor = a.scale * LOG2E / f1 / f2;
   o.lim = !valid ? -1 : (a.tree ? past - 1 : past + i);
   o.bits = valid && a.tree ? a.tree[(int64_t)b * a.S + i] : 0;
 }
 
-// Two e-th codes of words a and b interleaved: prmt selectors for codes 0, 1
-// and codes 2, 3 of both.
-constexpr uint32_t PAIR01 = 0x5140, PAIR23 = 0x7362;
+// Codes as f16 pairs, exactly. int8: the bits of 1024 + (c + 128) minus 1152 (the
+// mask, the exponent and the sign flip are one three-input operation); e4m3: the
+// hardware's conversion (cached rows never hold a NaN code).
+__device__ __forceinline__ uint32_t pair_int8(uint32_t codes02) {  // codes in bytes 0 and 2
+  const uint32_t u = (codes02 & 0x00ff00ffu) ^ 0x64806480u;
+  return b2m::h2_as_u32(__hsub2(b2m::u32_as_h2(u), __half2half2(__ushort_as_half(0x6480))));
+}
+__device__ __forceinline__ uint32_t pair_e4m3(uint32_t codes01) {  // codes in bytes 0 and 1
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(codes01));
+  return r;
+}
+__device__ __forceinline__ uint32_t pair_e4m3_hi(uint32_t codes23) {  // codes in bytes 2 and 3
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(codes23));
+  return r;
+}
 
-// Word of four codes c0 .. c3 -> (c0, c1) and (c2, c3) as f16 pairs. int8:
-// exact values, by the bits of 1024 + (c + 128) minus 1152. e4m3: exactly 2^-8
-// of the value, by moving the exponent and mantissa fields into place (every
-// bit pattern gives a finite number; the factor is folded into the scales).
+// Word of four codes c0 .. c3 as two pairs: (c0, c1) and (c2, c3) for e4m3, (c0,
+// c2) and (c1, c3) for int8 (what each takes the fewest operations for).
 template <bool E4M3>
-__device__ __forceinline__ void expand4(uint32_t w, uint32_t &p01, uint32_t &p23) {
+__device__ __forceinline__ void expand4(uint32_t w, uint32_t &p, uint32_t &q) {
   if (E4M3) {
-    const uint32_t a = b2m::prmt(w, 0u, 0x1404), b = b2m::prmt(w, 0u, 0x3424);
-    p01 = ((a >> 1) & 0x3f803f80u) | (a & 0x80008000u);
-    p23 = ((b >> 1) & 0x3f803f80u) | (b & 0x80008000u);
+    p = pair_e4m3(w);
+    q = pair_e4m3_hi(w);
   } else {
-    const uint32_t x = w ^ 0x80808080u;
-    const __half2 k = __half2half2(__ushort_as_half(0x6480));  // 1152
-    p01 = b2m::h2_as_u32(__hsub2(b2m::u32_as_h2(b2m::prmt(x, 0x64646464u, 0x4140)), k));
-    p23 = b2m::h2_as_u32(__hsub2(b2m::u32_as_h2(b2m::prmt(x, 0x64646464u, 0x4342)), k));
+    p = pair_int8(w);
+    q = pair_int8(w >> 8);
   }
 }
+// The order of a word's four values in expand4's pairs: position k holds value
+// expand_order<E4M3>(k).
 template <bool E4M3>
-__host__ __device__ constexpr float code_factor() {
-  return E4M3 ? 256.f : 1.f;
+__host__ __device__ constexpr int expand_order(int k) {
+  return E4M3 ? k : (k == 1 ? 2 : (k == 2 ? 1 : k));
+}
+
+// Words a, b of four codes each -> pairs (a_k, b_k), k = 0 .. 3.
+template <bool E4M3>
+__device__ __forceinline__ void expand_zip(uint32_t a, uint32_t b, uint32_t (&p)[4]) {
+  if (E4M3) {
+    const uint32_t x = b2m::prmt(a, b, 0x5140), y = b2m::prmt(a, b, 0x7362);  // a0 b0 a1 b1, a2 b2 a3 b3
+    p[0] = pair_e4m3(x), p[1] = pair_e4m3_hi(x);
+    p[2] = pair_e4m3(y), p[3] = pair_e4m3_hi(y);
+  } else {
+    const uint32_t x = b2m::prmt(a, b, 0x5410), y = b2m::prmt(a, b, 0x7632);  // a0 a1 b0 b1, a2 a3 b2 b3
+    p[0] = pair_int8(x), p[1] = pair_int8(x >> 8);
+    p[2] = pair_int8(y), p[3] = pair_int8(y >> 8);
+  }
 }
 
 }  // namespace kv8
