@@ -112,6 +112,7 @@ __device__ __forceinline__ void tmem_ld32x2(uint32_t taddr, f32x2 *v) {
 // polling took half of the issue slots. Gives up when another thread has, or
 // after two seconds (and records the error).
 __device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int32_t *dev_err) {
+#pragma unroll 1
   for (int i = 0; i < 2000; i++) {
     uint32_t ok;
     asm volatile(
@@ -204,6 +205,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   }
   if (warp == 8) tmem_alloc(slot, 256);
 
+#pragma unroll 1
   for (int rr = warp * 4 + (lane >> 3); rr < FL_ROWS; rr += FL_THREADS / 8) {
     QRow<D> q;
     load_q_row<D>(a, b, kvh, G, row0 + rr, past, q);
@@ -330,6 +332,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
       if (ntile > 1) load_k(1);
     }
     // K_{t+1} before V_t: its products are wanted first (under tile t's softmax).
+#pragma unroll 1
     for (int t = 0; t < ntile; t++) {
       if (t + 1 < ntile) {
         if (!put_k(t + 1)) break;
@@ -379,6 +382,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         tc_fence_after();
         issue_s(0);
       }
+#pragma unroll 1
       for (int t = 0; ok && t < ntile; t++) {
         if (t + 1 < ntile) {
           const int st = (t + 1) % L::KST;
@@ -421,6 +425,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     const int all_see = a.tree ? past : past + row0 / G + 1;  // keys below this are seen by every row
     float m = -INFINITY, mref = 0.f, l = 0.f;
     bool ok = true;
+#pragma unroll 1
     for (int t = 0; t < ntile; t++) {
       const int sl = t % FL_SLOTS, j0 = (t0 + t) * FL_TILE;
       ok = warp_wait_phase(s_full + (t & 1), (uint32_t)(t >> 1) & 1u, abort_flag, a.err);
@@ -592,6 +597,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   // Rows to memory, a cluster's ranks sharing them.
   const float *o_s = reinterpret_cast<const float *>(smem);
   constexpr int D4 = D / 4;
+#pragma unroll 1
   for (int e = rank * FL_THREADS + tid; e < FL_ROWS * D4; e += CL * FL_THREADS) {
     const int rr = e / D4, c = e % D4, r = row0 + rr;
     if (r >= nrows || *abort_flag) continue;

@@ -57,6 +57,14 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+// D += A . B (m16n8k16, f16 operands, fp32 sums). Not volatile, so that the
+// compiler may interleave independent products.
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 // How a row of D codes is dealt to the lanes: K rows in NKC chunks of KC bytes
 // for each of four lanes, V rows in NVC chunks of VC bytes for each of eight.
 template <int D>
@@ -115,26 +123,38 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
   const uint8_t *kcodes = a.kc + base * D, *vcodes = a.vc + base * D;
   const float *kscale = a.ks + base, *vscale = a.vs + base;
   const int ntile = (jend - jbeg + 15) >> 4;
+  const uint8_t *kp0 = kcodes + (int64_t)(jbeg + g) * D + t * L::KC;
+  const uint8_t *vp0 = vcodes + (int64_t)(jbeg + 2 * t) * D + g * L::VC;
+  // lane t of a group: K scale of keys g, g + 8, V scale of keys g, g + 8
+  const float *sp0 = (t & 2 ? vscale : kscale) + jbeg + g + 8 * (t & 1);
   auto issue = [&](int tile, int slot) {
     if (tile < ntile) {
-      const int j0 = jbeg + 16 * tile;
       uint8_t *s = ring + slot * L::SLOT;
+      const uint8_t *kp = kp0 + (int64_t)tile * (16 * D), *vp = vp0 + (int64_t)tile * (16 * D);
+      const float *sp = sp0 + 16 * tile;
+      // distances to the tile's other rows; in the last tile no further than its last row
+      int kd = 8 * D, vd[4] = {0, D, 8 * D, 9 * D};  // keys 2t, 2t+1, 2t+8, 2t+9
+      const int over = jbeg + 16 * tile + 16 - jend;
+      if (over > 0) {
+        const int left = 15 - over;  // index of the last row
+        kp += (int64_t)min(0, left - g) * D;
+        kd = (min(left, g + 8) - min(left, g)) * D;
+        const int k0 = min(left, 2 * t);
+        vp += (int64_t)(k0 - 2 * t) * D;
 #pragma unroll
-      for (int hf = 0; hf < 2; hf++) {
-        const uint8_t *src = kcodes + (int64_t)min(j0 + 8 * hf + g, jend - 1) * D + t * L::KC;
+        for (int q = 1; q < 4; q++) vd[q] = (min(left, 2 * t + (q & 1) + 8 * (q >> 1)) - k0) * D;
+        sp += min(0, left - g - 8 * (t & 1));
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++)
 #pragma unroll
         for (int c = 0; c < L::NKC; c++)
-          cp_async<L::KC>(s + ((hf * L::NKC + c) * 32 + lane) * L::KC, src + c * 4 * L::KC);
-      }
+          cp_async<L::KC>(s + ((hf * L::NKC + c) * 32 + lane) * L::KC, kp + hf * kd + c * 4 * L::KC);
 #pragma unroll
-      for (int q = 0; q < 4; q++) {  // keys 2t, 2t+1, 2t+8, 2t+9
-        const uint8_t *src = vcodes + (int64_t)min(j0 + 2 * t + (q & 1) + 8 * (q >> 1), jend - 1) * D + g * L::VC;
+      for (int q = 0; q < 4; q++)
 #pragma unroll
         for (int c = 0; c < L::NVC; c++)
-          cp_async<L::VC>(s + L::K_BYTES + ((q * L::NVC + c) * 32 + lane) * L::VC, src + c * 8 * L::VC);
-      }
-      // lane t of a group: K scale of keys g, g + 8, V scale of keys g, g + 8
-      const float *sp = (t & 2 ? vscale : kscale) + min(j0 + g + 8 * (t & 1), jend - 1);
+          cp_async<L::VC>(s + L::K_BYTES + ((q * L::NVC + c) * 32 + lane) * L::VC, vp + vd[q] + c * 8 * L::VC);
       cp_async<4>(s + L::K_BYTES + L::V_BYTES + lane * 4, sp);
     }
     cp_commit();
@@ -155,6 +175,7 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
   {
     const int i0 = max(0, jbeg - past), i1 = !fused_append ? i0 : (rank == CL - 1 ? a.S : min(a.S, jend - past));
     const int nnew = 2 * max(0, i1 - i0);
+#pragma unroll 1
     for (int it = warp; it < nnew + R / 4; it += ST_WARPS) {
       if (it < nnew) {
         append_side_vec<E4M3, (D + 127) / 128>(a, b, i0 + (it >> 1), kvh, it & 1, a.past[b], lane);
@@ -210,6 +231,7 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
   const int all_see = a.tree ? past : past + row0 / G + 1;  // keys below this are seen by every row
 
   int slot = 0;
+#pragma unroll 1
   for (int tile = warp; tile < ntile; tile += ST_WARPS) {
     cp_wait<ST_STAGES - 2>();
     __syncwarp();
@@ -217,11 +239,11 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
     const uint8_t *s = ring + slot * L::SLOT;
     const int j0 = jbeg + 16 * tile;
     // S^T = K . Q^T
-    float c[NT][4], cl[NT][4];  // (two chains of products: half the latency)
+    float c[NT][4], ch[2][NT][4], cl[2][NT][4];  // (four chains of products)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int u = 0; u < 4; u++) c[nt][u] = cl[nt][u] = 0.f;
+      for (int u = 0; u < 4; u++) ch[0][nt][u] = ch[1][nt][u] = cl[0][nt][u] = cl[1][nt][u] = 0.f;
 #pragma unroll
     for (int cc = 0; cc < L::NKC; cc++) {
       uint32_t w0[L::KW], w1[L::KW];
@@ -243,11 +265,15 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
           const uint4 q = qfrag[(nt * L::KSTEPS + cc * L::KW + w) * 32 + lane];
-          b2m::mma_16816(c[nt], A, q.x, q.y, c[nt]);
-          b2m::mma_16816(cl[nt], A, q.z, q.w, cl[nt]);
+          mma(ch[w & 1][nt], A, q.x, q.y);
+          mma(cl[w & 1][nt], A, q.z, q.w);
         }
       }
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int u = 0; u < 4; u++) c[nt][u] = (ch[0][nt][u] + ch[1][nt][u]) + (cl[0][nt][u] + cl[1][nt][u]);
     // Scores in log2 units; masked ones -inf.
     const float4 sc = *reinterpret_cast<const float4 *>(s + L::K_BYTES + L::V_BYTES + g * 16);
     float x[NT][2][2];  // [key g, g + 8][row 2t, 2t + 1]
@@ -255,8 +281,8 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        x[nt][0][u] = (c[nt][u] + cl[nt][u]) * sc.x * rf[nt][u];
-        x[nt][1][u] = (c[nt][2 + u] + cl[nt][2 + u]) * sc.y * rf[nt][u];
+        x[nt][0][u] = c[nt][u] * sc.x * rf[nt][u];
+        x[nt][1][u] = c[nt][2 + u] * sc.y * rf[nt][u];
       }
     const bool whole = j0 + 16 <= min(jend, all_see);
     uint32_t seen = 0xffffffffu;  // bit (nt * 2 + key) * 2 + row
@@ -362,11 +388,11 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
 #pragma unroll
         for (int hf = 0; hf < 2; hf++)
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            float *acc = o[nt][(cc * L::VW + w) * 2 + hf];
-            b2m::mma_16816(acc, A[hf], bh[nt][0], bh[nt][1], acc);
-            b2m::mma_16816(acc, A[hf], bl[nt][0], bl[nt][1], acc);
-          }
+          for (int nt = 0; nt < NT; nt++) mma(o[nt][(cc * L::VW + w) * 2 + hf], A[hf], bh[nt][0], bh[nt][1]);
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) mma(o[nt][(cc * L::VW + w) * 2 + hf], A[hf], bl[nt][0], bl[nt][1]);
       }
     }
     slot = slot + 1 == ST_STAGES ? 0 : slot + 1;
@@ -404,6 +430,7 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
     return sl == 0.f ? 0.f : (sm == -INFINITY ? 1.f : ex2(sm - top));
   };
   constexpr int D4 = D / 4;
+#pragma unroll 1
   for (int e = tid; e < R * D4; e += ST_THREADS) {
     const int rr = e / D4;
     float top = -INFINITY, sum = 0.f;
@@ -427,6 +454,7 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
     cluster.sync();
   else
     __syncthreads();
+#pragma unroll 1
   for (int e = rank * ST_THREADS + tid; e < R * D4; e += CL * ST_THREADS) {
     const int rr = e / D4, r = row0 + rr;
     if (r >= nrows) continue;
@@ -460,12 +488,23 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   constexpr auto kern = kv8_step_kernel<E4M3, D, NT>;
   b2m::set_smem_limit_once<kern>(M::BYTES);
   const int nrows = a.S * (a.H / a.KVH), tiles = (nrows + M::R - 1) / M::R;
-  const bool fused = tiles == 1 && append_rows_vec(a);
+  // One new row per sequence is appended beside the query rows; more would hold up
+  // the CTA whose range they fall into (eight: 7 us longer than a launch of its own).
+  const bool fused = a.S == 1 && tiles == 1 && append_rows_vec(a);
   if (!fused) launch_kv8_append(a, s);
-  // Key splits: CTAs for four per SM, at least 64 cache positions each.
+  // Key splits. A CTA costs some 8 us however few keys it has, and a cluster is
+  // only placed where all its CTAs fit, so a split has to pay for itself: up to one
+  // wave of CTAs that are resident together (three per SM for 8 query rows, two for
+  // 16), at least 128 cache positions each, 16 CTAs at most; and two for calls of
+  // between one and two waves of long rows, whose second wave would be mostly
+  // empty (64 sequences over 4096 .. 8191 positions: 179 us, 208 unsplit; 32 trees
+  // over 1500: 45 us unsplit, 61 and 66 with two and four).
   const int64_t ctas = (int64_t)a.B * a.KVH * tiles;
+  const int64_t wave = (NT == 1 ? 3 : 2) * (int64_t)b2m::device_sm_count();
   int cl = 1;
-  while (cl < 8 && ctas * cl < 4 * b2m::device_sm_count() && a.CAP > 64 * cl) cl *= 2;
+  while (cl < 16 && ctas * cl * 2 <= wave && a.CAP >= 256 * cl) cl *= 2;
+  if (cl == 1 && NT == 1 && ctas > wave && ctas < 2 * wave && a.CAP >= 2048) cl = 2;
+  b2m::allow_large_cluster_once<kern>();
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * cl), (unsigned)a.KVH, (unsigned)a.B);
   cfg.blockDim = dim3(ST_THREADS);
