@@ -564,7 +564,8 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     // longer read (the last products have completed).
     float *ost = reinterpret_cast<float *>(smem) + rr * L::OST;
     if (ok) {
-      const float vo = ntile > 0 ? *vref_s : 0.f;
+      // (alone, a CTA divides here; a row that saw nothing: zeros)
+      const float vo = ntile == 0 ? 0.f : (CL > 1 ? *vref_s : (l == 0.f ? 0.f : *vref_s / l));
 #pragma unroll
       for (int c = 0; c < D / 16; c++) {
         uint32_t u[16];
@@ -603,12 +604,10 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     if (r >= nrows || *abort_flag) continue;
     const float *src = o_s + rr * L::OST + 4 * c;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
     if (CL == 1) {
       acc = *reinterpret_cast<const float4 *>(src);
-      sum = row_l[rr];
     } else {
-      float top = -INFINITY;
+      float top = -INFINITY, sum = 0.f;
       for (int q = 0; q < CL; q++) top = fmaxf(top, *cluster.map_shared_rank(row_m + rr, q));
       for (int q = 0; q < CL; q++) {
         const float sl = *cluster.map_shared_rank(row_l + rr, q), sm = *cluster.map_shared_rank(row_m + rr, q);
@@ -618,9 +617,9 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         sum += sl * f;
         acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
       }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that saw nothing: zeros
-    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
     const int64_t at = ((int64_t)b * a.S + r / G) * a.H * D + (int64_t)(kvh * G + r % G) * D + 4 * c;
     if (a.out) *reinterpret_cast<float4 *>(a.out + at) = acc;
     if (a.out16) {

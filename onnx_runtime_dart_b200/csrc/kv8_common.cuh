@@ -468,25 +468,39 @@ __device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int
     for (int f = 1; f < 8; f <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, f);
     inv = 1.f / sqrtf(ss / D + (float)a.eps);
   }
-  float mx = 0.f;
+  if (gain) {
 #pragma unroll
-  for (int u = 0; u < NC; u++) {
-    const int d = 4 * (l8 + 8 * u);
-    float x[4] = {o.v[u].x, o.v[u].y, o.v[u].z, o.v[u].w};
-    if (gain) {
-      const float4 g4 = *reinterpret_cast<const float4 *>(gain + d);
-      x[0] *= inv * g4.x, x[1] *= inv * g4.y, x[2] *= inv * g4.z, x[3] *= inv * g4.w;
+    for (int u = 0; u < NC; u++) {
+      const float4 g4 = *reinterpret_cast<const float4 *>(gain + 4 * (l8 + 8 * u));
+      o.v[u].x *= inv * g4.x, o.v[u].y *= inv * g4.y, o.v[u].z *= inv * g4.z, o.v[u].w *= inv * g4.w;
     }
-    if (turn && d < a.rot) {
+  }
+  if (turn && a.rot == D && !a.interleaved && NC % 2 == 0) {
+    // The whole head in halves: a chunk's partner is NC / 2 chunks on, in this lane.
+#pragma unroll
+    for (int u = 0; u < NC / 2; u++) {
+      const int64_t at = pos * a.half + 4 * (l8 + 8 * u);
+      const float4 c = *reinterpret_cast<const float4 *>(a.cos + at), n = *reinterpret_cast<const float4 *>(a.sin + at);
+      const float4 x = o.v[u], y = o.v[u + NC / 2];
+      o.v[u] = make_float4(x.x * c.x - y.x * n.x, x.y * c.y - y.y * n.y, x.z * c.z - y.z * n.z, x.w * c.w - y.w * n.w);
+      o.v[u + NC / 2] =
+          make_float4(y.x * c.x + x.x * n.x, y.y * c.y + x.y * n.y, y.z * c.z + x.z * n.z, y.w * c.w + x.w * n.w);
+    }
+  } else if (turn) {
+#pragma unroll
+    for (int u = 0; u < NC; u++) {
+      const int d = 4 * (l8 + 8 * u);
+      if (d >= a.rot) continue;
+      const float x[4] = {o.v[u].x, o.v[u].y, o.v[u].z, o.v[u].w};
       const bool first = a.interleaved || d < hr;
-      float c[4], sn[4], w[4];
+      float c[4], sn[4], w[4], y[4];
       if (a.interleaved) {
         const float2 c2 = *reinterpret_cast<const float2 *>(a.cos + pos * a.half + (d >> 1));
         const float2 s2 = *reinterpret_cast<const float2 *>(a.sin + pos * a.half + (d >> 1));
         c[0] = c[1] = c2.x, c[2] = c[3] = c2.y;
         sn[0] = s2.x, sn[1] = -s2.x, sn[2] = s2.y, sn[3] = -s2.y;
         w[0] = x[1], w[1] = x[0], w[2] = x[3], w[3] = x[2];
-      } else {
+      } else {  // the partner from memory again
         const int pi = first ? d : d - hr, e = first ? d + hr : d - hr;
         const float4 c4 = *reinterpret_cast<const float4 *>(a.cos + pos * a.half + pi);
         const float4 s4 = *reinterpret_cast<const float4 *>(a.sin + pos * a.half + pi);
@@ -501,10 +515,15 @@ __device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int
         w[0] = w4.x, w[1] = w4.y, w[2] = w4.z, w[3] = w4.w;
       }
 #pragma unroll
-      for (int k = 0; k < 4; k++) x[k] = x[k] * c[k] - w[k] * sn[k];
+      for (int k = 0; k < 4; k++) y[k] = x[k] * c[k] - w[k] * sn[k];
+      o.v[u] = make_float4(y[0], y[1], y[2], y[3]);
     }
-    o.v[u] = valid ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+  }
+  float mx = 0.f;
+#pragma unroll
+  for (int u = 0; u < NC; u++) {
+    if (!valid) o.v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(o.v[u].x), fabsf(o.v[u].y)), fmaxf(fabsf(o.v[u].z), fabsf(o.v[u].w))));
   }
 #pragma unroll
   for (int f = 1; f < 8; f <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, f));
