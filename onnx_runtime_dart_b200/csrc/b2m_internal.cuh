@@ -7,6 +7,7 @@
 
 #include <string>
 #include <unordered_map>
+#include <vector>
 
 #include "../../include/b2m.h"
 
@@ -66,6 +67,10 @@ struct b2m_ctx {
   // operands). Stream-ordered: reused by the next op on the same stream.
   void *scratch = nullptr;
   size_t scratch_bytes = 0;
+  // A stream capture has recorded launches on the current workspace: it then
+  // outlives its replacement (replays keep using it), until the context closes.
+  bool scratch_in_graph = false;
+  std::vector<void *> retired_scratch;
   // The error word that kernels with bounded spin-waits (and index checks)
   // set: mapped pinned host memory, so a synchronising call reads it with a
   // plain load instead of a device-to-host copy. dev_err is its device

@@ -165,14 +165,22 @@ struct Scratch {
   b2m_ctx *ctx;
   size_t used = 0;
   explicit Scratch(b2m_ctx *c, size_t need) : ctx(c) {
-    if (need > 0 && need > ctx->scratch_bytes) {
-      if (ctx->scratch) B2M_CUDA(cudaFreeAsync(ctx->scratch, ctx->stream));
+    if (need == 0) return;
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    B2M_CUDA(cudaStreamIsCapturing(ctx->stream, &cs));
+    if (need > ctx->scratch_bytes) {
+      if (ctx->scratch && ctx->scratch_in_graph)
+        ctx->retired_scratch.push_back(ctx->scratch);
+      else if (ctx->scratch)
+        B2M_CUDA(cudaFreeAsync(ctx->scratch, ctx->stream));
       ctx->scratch = nullptr;
       ctx->scratch_bytes = 0;
+      ctx->scratch_in_graph = false;
       const size_t sz = std::max(need, (size_t)1 << 20);
       B2M_CUDA(cudaMallocAsync(&ctx->scratch, sz, ctx->stream));
       ctx->scratch_bytes = sz;
     }
+    if (cs == cudaStreamCaptureStatusActive) ctx->scratch_in_graph = true;
   }
   void *take(size_t bytes) {
     const size_t off = (used + 255) & ~(size_t)255;
@@ -789,6 +797,7 @@ B2M_API b2m_status b2m_shutdown(b2m_ctx *ctx) {
     cudaStreamSynchronize(ctx->stream);
     cudaStreamSynchronize(ctx->own_stream);
     if (ctx->scratch) cudaFreeAsync(ctx->scratch, ctx->own_stream);
+    for (void *p : ctx->retired_scratch) cudaFreeAsync(p, ctx->own_stream);
     cudaStreamSynchronize(ctx->own_stream);
     if (ctx->pinned) cudaFreeHost(ctx->pinned);
     if (ctx->err_host) cudaFreeHost(ctx->err_host);

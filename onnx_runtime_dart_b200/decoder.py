@@ -80,6 +80,33 @@ def swiglu_row_order(inter: int) -> np.ndarray:
     return np.concatenate([t, t + inter], axis=1).reshape(-1)
 
 
+def tree_arrays(parents):
+    """(bits, depth) of a drafted tree as b2m_gqa_kv8_dev takes them, from each
+    node's parent: node 0 is the root (parent -1), every other node's parent
+    comes before it. bits[i] holds node i and its ancestors, depth[i] its
+    distance from the root."""
+    bits, depth = [], []
+    for i, p in enumerate(parents):
+        if (i == 0) != (p < 0) or p >= i:
+            raise N.ArgumentError("drafted tree: node 0 is the root and parents come before their children")
+        bits.append((1 << i) | (bits[p] if i else 0))
+        depth.append(depth[p] + 1 if i else 0)
+    return bits, depth
+
+
+def accepted_path(tokens, parents, greedy):
+    """Nodes of a drafted tree that greedy decoding would have produced: from
+    the root on, the child (the first, if several) that holds the token the
+    model chose after its parent."""
+    path = [0]
+    while True:
+        want = greedy[path[-1]]
+        nxt = next((i for i in range(path[-1] + 1, len(tokens)) if parents[i] == path[-1] and tokens[i] == want), None)
+        if nxt is None:
+            return path
+        path.append(nxt)
+
+
 def _ptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.data_ptr())
 
@@ -90,7 +117,8 @@ class Int4Decoder:
 
     def __init__(self, ctx, cfg: DecoderConfig, batch: int, cap: int, max_prefill: int, seed: int = 0,
                  keep_host: bool = False, mode: int = N.MODE_FAST, fused: bool = True, session=None,
-                 producer_f16: bool = True, fold_qk_norm: bool = True, swiglu_epilogue: bool = True):
+                 producer_f16: bool = True, fold_qk_norm: bool = True, swiglu_epilogue: bool = True,
+                 kv_type: str | None = None):
         import torch
 
         if mode not in (N.MODE_FAST, N.MODE_PRECISE, N.MODE_EXACT):
@@ -127,6 +155,15 @@ class Int4Decoder:
         # tensor-core route from the GEMM's epilogue: no gate / up rows in
         # memory and no SiLU*Mul launch, the same results.
         self.swiglu = bool(swiglu_epilogue and self.fused and session is None and cfg.inter % 64 == 0)
+        # kv_type: None keeps the reference's fp32 KV cache; "int8" or "e4m3" an
+        # 8-bit one with a scale per cached row (a quarter of the bytes), whose
+        # attention call normalises, rotates, quantises and appends by itself
+        # and also takes drafted trees (verify).
+        if kv_type not in (None, "int8", "e4m3"):
+            raise N.ArgumentError("decoder: kv_type must be None, 'int8' or 'e4m3'")
+        self.kv_type = kv_type
+        self._tree = None    # (bits, depth) device tensors while a drafted tree runs
+        self._report = None  # buffers of b2m_logprobs_dev for decode(top_logprobs=)
         self._routes = {}
         self.torch = torch
         self.ctx, self.cfg, self.B, self.cap = ctx, cfg, batch, cap
@@ -145,8 +182,16 @@ class Int4Decoder:
         self.cos = torch.from_numpy(np.cos(ang).astype(np.float32)).to(dev)
         self.sin = torch.from_numpy(np.sin(ang).astype(np.float32)).to(dev)
         kv_shape = (c.layers, batch, c.kv_heads, cap, c.head_dim)
-        self.kcache = torch.zeros(kv_shape, device=dev, dtype=torch.float32)
-        self.vcache = torch.zeros(kv_shape, device=dev, dtype=torch.float32)
+        kv_dtype = torch.float32 if kv_type is None else torch.uint8
+        self.kcache = torch.zeros(kv_shape, device=dev, dtype=kv_dtype)
+        self.vcache = torch.zeros(kv_shape, device=dev, dtype=kv_dtype)
+        if kv_type is not None:
+            self.kscale = torch.zeros(kv_shape[:-1], device=dev, dtype=torch.float32)
+            self.vscale = torch.zeros(kv_shape[:-1], device=dev, dtype=torch.float32)
+            code = N.B2M_INT8 if kv_type == "int8" else N.B2M_FLOAT8E4M3FN
+            self.kv8 = [N.Kv8Cache(self.kcache[li].data_ptr(), self.vcache[li].data_ptr(), self.kscale[li].data_ptr(),
+                                   self.vscale[li].data_ptr(), code, batch, c.kv_heads, cap, c.head_dim)
+                        for li in range(c.layers)]
         self.past = torch.zeros(batch, device=dev, dtype=torch.int32)
         t = batch * max_prefill
         self.max_tokens = t
@@ -271,7 +316,8 @@ class Int4Decoder:
 
     @classmethod
     def from_onnx(cls, ctx, path: str, cfg: DecoderConfig, batch: int, cap: int, max_prefill: int,
-                  mode: int = N.MODE_FAST, cache_dir: str | None = None) -> "Int4Decoder":
+                  mode: int = N.MODE_FAST, cache_dir: str | None = None,
+                  kv_type: str | None = None) -> "Int4Decoder":
         """A decoder over a model written by export_onnx: load_model reads it,
         prepack_session packs every MatMulNBits / MatMul initializer under the
         keys GpuDispatch looks up (and declares the projections' order for the
@@ -284,7 +330,7 @@ class Int4Decoder:
         model = load_model(path)
         disp, _ = prepack_session(ctx, model, cache_dir=cache_dir, nbits_mode=mode)
         sess = _OnnxSession(model, disp, cfg)
-        return cls(ctx, cfg, batch, cap, max_prefill, mode=mode, session=sess)
+        return cls(ctx, cfg, batch, cap, max_prefill, mode=mode, session=sess, kv_type=kv_type)
 
     def _dispatch_proj(self, part: str, lw, x, T: int, y):
         """One MatMulNBits node through the dispatch, into buffer y."""
@@ -388,11 +434,49 @@ class Int4Decoder:
         sequence's last token in self.logits and its argmax in self.next_ids,
         and advances past by seq. Everything is enqueued on the context's
         stream."""
+        self._hidden(seq)
+        self._last_rows(seq)
+
+    def _hidden(self, seq: int):
+        """The layers and the final norm: the rows of all B*seq tokens in self.h."""
         self.ctx.set_attention_mode(N.MODE_EXACT if self.mode == N.MODE_EXACT else N.MODE_FAST)
         try:
             self._layers(seq, self.B * seq)
         finally:
             self.ctx.set_attention_mode(N.MODE_FAST)
+
+    def _head(self, idx, T: int):
+        """Logits of the B rows `idx` (int64, device) of self.h, into self.logits."""
+        lib, h = self.lib, self.ctx.handle
+        N.check(lib.b2m_gather_rows_dev(h, _ptr(self.h), _ptr(idx), _ptr(self.last), self.B, T, self.cfg.hidden))
+        y = ctypes.c_void_p(self.t_logits.handle.value)
+        lm_mode = N.MODE_EXACT if self.mode == N.MODE_EXACT else N.MODE_FAST
+        N.check(lib.b2m_matmul_f32(h, self.t_last.handle, None, self.lm_head.handle, lm_mode, ctypes.byref(y)))
+
+    def _last_rows(self, seq: int):
+        """Logits and argmax of each sequence's last token; past moves on."""
+        lib, h, V = self.lib, self.ctx.handle, self.cfg.vocab
+        idx = self.last_idx.get(seq)
+        if idx is None:
+            idx = self.torch.arange(self.B, device=self.dev, dtype=self.torch.int64) * seq + (seq - 1)
+            self.last_idx[seq] = idx
+        self._head(idx, self.B * seq)
+        N.check(lib.b2m_argmax_dev(h, _ptr(self.logits), _ptr(self.next_ids), self.B, V))
+        if self._report is not None:
+            lp, ent, top, top_lp = self._report
+            N.check(lib.b2m_logprobs_dev(h, _ptr(self.logits), V, _ptr(self.next_ids), self.B, V, _ptr(lp), _ptr(ent),
+                                         top.shape[1], _ptr(top) if top.shape[1] else None,
+                                         _ptr(top_lp) if top.shape[1] else None))
+        N.check(lib.b2m_advance_positions_dev(h, _ptr(self.past), self.B, seq))
+
+    def _all_rows(self, T: int, each):
+        """Calls each(first, count) with the logits of rows first .. first + count - 1
+        of self.h in self.logits, B rows at a time (the last rows are repeated
+        to fill the last call)."""
+        for r0 in range(0, T, self.B):
+            idx = self.torch.arange(r0, r0 + self.B, device=self.dev, dtype=self.torch.int64).clamp_(max=T - 1)
+            self._head(idx, T)
+            each(r0, min(self.B, T - r0))
 
     def _f16_input(self, w, T: int) -> bool:
         """Whether the fused projection `w` at T rows takes its activations as
@@ -453,7 +537,7 @@ class Int4Decoder:
             self._down_f16 = dn16
             # (with the folded head norms the attention writes only the o
             # projection's f16 operand when that is what it reads)
-            self._o_f16 = o16 and self.fold_qk_norm
+            self._o_f16 = o16 and (self.fold_qk_norm or self.kv_type is not None)
             if li == 0:
                 self._norm(self.res, None, lw["attn_norm"], None, T, qkv16)
             else:  # residual of the previous layer's MLP, then the attention norm
@@ -471,7 +555,15 @@ class Int4Decoder:
                                                      _ptr(getattr(self, part))))
                 qp, kp, vp = self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr()
                 q_rs, kv_rs = c.heads * D, c.kv_heads * D
-            if self.fused and self.fold_qk_norm:  # head norms inside the attention call
+            if self.kv_type is not None:  # head norms, rotary, quantisation and append inside the attention call
+                bits, depth = self._tree or (None, None)
+                chk(lib.b2m_gqa_kv8_dev(h, ctypes.byref(self.kv8[li]), ctypes.c_void_p(qp), ctypes.c_void_p(kp),
+                                        ctypes.c_void_p(vp), q_rs, kv_rs, _ptr(lw["qk_gain"]), c.eps, _ptr(self.past),
+                                        None if bits is None else _ptr(bits), None if depth is None else _ptr(depth),
+                                        _ptr(self.cos), _ptr(self.sin), D // 2, D, 0,
+                                        None if o16 else _ptr(self.attn), _ptr(self.attn16) if o16 else None, seq,
+                                        c.heads, 0.0))
+            elif self.fused and self.fold_qk_norm:  # head norms inside the attention call
                 chk(lib.b2m_gqa_qknorm_dev(h, ctypes.c_void_p(qp), ctypes.c_void_p(kp), ctypes.c_void_p(vp), q_rs,
                                            kv_rs, _ptr(lw["qk_gain"]), c.eps, _ptr(self.kcache[li]),
                                            _ptr(self.vcache[li]), _ptr(self.past), _ptr(self.cos), _ptr(self.sin),
@@ -531,16 +623,6 @@ class Int4Decoder:
                 self._proj(lw["down"], T, dn16, self.act, getattr(self, "act16", None), self.down)
         chk(lib.b2m_rmsnorm_dev(h, _ptr(self.down), _ptr(self.res), _ptr(self.final_norm), _ptr(self.h),
                                 _ptr(self.res), T, H, c.eps))
-        idx = self.last_idx.get(seq)
-        if idx is None:
-            idx = self.torch.arange(self.B, device=self.dev, dtype=self.torch.int64) * seq + (seq - 1)
-            self.last_idx[seq] = idx
-        chk(lib.b2m_gather_rows_dev(h, _ptr(self.h), _ptr(idx), _ptr(self.last), self.B, T, H))
-        y = ctypes.c_void_p(self.t_logits.handle.value)
-        lm_mode = N.MODE_EXACT if self.mode == N.MODE_EXACT else N.MODE_FAST
-        chk(lib.b2m_matmul_f32(h, self.t_last.handle, None, self.lm_head.handle, lm_mode, ctypes.byref(y)))
-        chk(lib.b2m_argmax_dev(h, _ptr(self.logits), _ptr(self.next_ids), self.B, c.vocab))
-        chk(lib.b2m_advance_positions_dev(h, _ptr(self.past), self.B, seq))
 
     def prefill(self, prompt_ids) -> None:
         """prompt_ids: int64 [B][S] (host or device). Resets the cache positions,
@@ -559,12 +641,28 @@ class Int4Decoder:
         self.ids[: self.B].copy_(self.next_ids)
         self._forward(1)
 
-    def decode(self, steps: int, use_graph: bool = True):
+    def decode(self, steps: int, use_graph: bool = True, top_logprobs: int | None = None):
         """Greedy decode `steps` tokens (device-resident loop); returns the
-        generated ids as an int64 tensor [steps][B] on the device."""
+        generated ids as an int64 tensor [steps][B] on the device. With
+        top_logprobs = k (0 .. 32) it returns (ids, report): the chosen tokens'
+        log probabilities and the entropies [steps][B] under "logprob" and
+        "entropy", the k likeliest ids and their log probabilities
+        [steps][B][k] under "top_ids" and "top_logprobs"."""
         torch = self.torch
+        k = self._report[2].shape[1] if self._report is not None else None
+        if k != top_logprobs:  # another step: captured anew
+            if top_logprobs is not None and not 0 <= top_logprobs <= min(N.LOGPROBS_MAX_K, self.cfg.vocab):
+                raise N.ArgumentError("decoder decode: top_logprobs must lie in [0, 32]")
+            f32 = dict(device=self.dev, dtype=torch.float32)
+            self._report = None if top_logprobs is None else (
+                torch.empty(self.B, **f32), torch.empty(self.B, **f32),
+                torch.empty((self.B, top_logprobs), device=self.dev, dtype=torch.int64),
+                torch.empty((self.B, top_logprobs), **f32))
+            self.graph = None
         with torch_stream_scope(self.ctx, torch, self.stream) as stream:
             out = torch.empty((steps, self.B), device=self.dev, dtype=torch.int64)
+            report = None if self._report is None else [
+                torch.empty((steps, *t.shape), device=self.dev, dtype=t.dtype) for t in self._report]
             if use_graph and self.graph is None:
                 # Capture one step; a warm-up step first so every kernel
                 # attribute and scratch size is settled outside the capture.
@@ -589,6 +687,88 @@ class Int4Decoder:
                 else:
                     self._decode_body()
                 out[i].copy_(self.next_ids)
+                for dst, src in zip(report or (), self._report or ()):
+                    dst[i].copy_(src)
+        if report is None:
+            return out
+        return out, dict(zip(("logprob", "entropy", "top_ids", "top_logprobs"), report))
+
+    def score(self, ids):
+        """Log probabilities of the tokens ids [B][S] (int64, host or device)
+        given the tokens before them: (logprob, entropy), both [B][S - 1], entry
+        t for token t + 1. Resets the cache positions and runs the tokens as
+        prefill does."""
+        torch, lib, h, V = self.torch, self.lib, self.ctx.handle, self.cfg.vocab
+        ids = torch.as_tensor(ids, dtype=torch.int64).to(self.dev).reshape(-1)
+        seq = ids.numel() // self.B
+        if ids.numel() != self.B * seq or ids.numel() > self.max_tokens or seq > self.cap or seq < 1:
+            raise N.ArgumentError("decoder score: token shape does not fit the decoder")
+        T = ids.numel()
+        with torch_stream_scope(self.ctx, torch, self.stream):
+            self.past.zero_()
+            self.ids[:T].copy_(ids)
+            target = ids.view(self.B, seq).roll(-1, 1).reshape(-1)  # (each last row's is dropped below)
+            lp = torch.empty(T, device=self.dev, dtype=torch.float32)
+            ent = torch.empty_like(lp)
+            self._hidden(seq)
+
+            def each(r0, n):
+                N.check(lib.b2m_logprobs_dev(h, _ptr(self.logits), V, _ptr(target[r0:]), n, V, _ptr(lp[r0:]),
+                                             _ptr(ent[r0:]), 0, None, None))
+
+            self._all_rows(T, each)
+            self._last_rows(seq)
+            out = tuple(t.view(self.B, seq)[:, :-1].clone() for t in (lp, ent))
+        return out
+
+    def verify(self, tokens, parents):
+        """One speculative step over an 8-bit cache: runs a drafted tree of n
+        tokens for every sequence, keeps the part that greedy decoding would
+        have produced, and goes on behind it.
+
+        tokens: int64 [B][n], node 0 the token to be fed next (self.next_ids);
+        parents: [n] for all sequences or [B][n] (see tree_arrays; n <= 64).
+        Returns per sequence the list of tokens generated: the accepted drafts
+        and the token the model chose behind them, which is left in
+        self.next_ids. Synchronises with the host once."""
+        torch, lib, h, V = self.torch, self.lib, self.ctx.handle, self.cfg.vocab
+        if self.kv_type is None:
+            raise N.UnsupportedError("decoder verify: drafted trees need an 8-bit cache (kv_type)")
+        tokens = torch.as_tensor(tokens, dtype=torch.int64).cpu().reshape(self.B, -1)
+        n = tokens.shape[1]
+        par = torch.as_tensor(parents, dtype=torch.int64).cpu()
+        par = par.reshape(1, -1).expand(self.B, -1) if par.dim() == 1 else par
+        if n < 1 or n > 64 or par.shape != (self.B, n) or self.B * n > self.max_tokens:
+            raise N.ArgumentError("decoder verify: tree shape does not fit the decoder")
+        if int(tokens.min()) < 0 or int(tokens.max()) >= V:
+            raise N.ArgumentError("decoder verify: token outside the vocabulary")
+        trees = [tree_arrays(p) for p in par.tolist()]
+        signed = [[x - (1 << 64) if x >> 63 else x for x in b] for b, _ in trees]
+        T = self.B * n
+        with torch_stream_scope(self.ctx, torch, self.stream):
+            self.ids[:T].copy_(tokens.reshape(-1))
+            greedy = torch.empty(T + self.B, device=self.dev, dtype=torch.int64)
+            self._tree = (torch.tensor(signed, dtype=torch.int64).to(self.dev),
+                          torch.tensor([d for _, d in trees], dtype=torch.int32).to(self.dev))
+            try:
+                self._hidden(n)
+            finally:
+                self._tree = None
+
+            def each(r0, _):
+                N.check(lib.b2m_argmax_dev(h, _ptr(self.logits), _ptr(greedy[r0:]), self.B, V))
+
+            self._all_rows(T, each)
+            N.check(lib.b2m_synchronize(h))  # also reports a cache that was full
+            g = greedy[:T].cpu().view(self.B, n).tolist()
+            paths = [accepted_path(t, p, q) for t, p, q in zip(tokens.tolist(), par.tolist(), g)]
+            out = [[t[i] for i in path[1:]] + [q[path[-1]]] for t, q, path in zip(tokens.tolist(), g, paths)]
+            count = torch.tensor([len(p) for p in paths], dtype=torch.int32).to(self.dev)
+            path = torch.tensor([p + [0] * (n - len(p)) for p in paths], dtype=torch.int32).to(self.dev)
+            N.check(lib.b2m_kv8_keep_dev(h, ctypes.byref(self.kv8[0]), self.cfg.layers, _ptr(self.past), _ptr(path),
+                                         _ptr(count), n))
+            self.past.add_(count)
+            self.next_ids.copy_(torch.tensor([o[-1] for o in out], dtype=torch.int64))
         return out
 
 
