@@ -17,9 +17,10 @@
 // No cross-thread reduction is left in the softmax. Two CTAs share an SM, so one's
 // exponentials run under the other's products.
 //
-// SPLIT (an fp32 output is wanted): Q and P as two f16 terms each, two products
-// per operand pair, fp32 accuracy. Without it Q and P are rounded to f16 once,
-// an error below that of the f16 output's own rounding.
+// P is split into two f16 terms (22 bits, two products); so is Q (QS) where fp32
+// rows are wanted. For an f16 output alone Q is rounded to f16 once: an error like
+// that of the output's own rounding (against 64 bits 2.8e-4 in all, 2.1e-4 with
+// both split, 3.5e-4 with neither; 259, 281 and 250 us for 4 x 2048 tokens).
 //
 // Few row tiles over many keys (a tree on long sequences): the CTAs of a cluster
 // split the keys and merge their O, m and l through distributed shared memory in
@@ -135,12 +136,12 @@ __device__ __forceinline__ bool warp_wait_phase(uint64_t *bar, uint32_t parity, 
   return __all_sync(0xffffffffu, wait_phase(bar, parity, abort_flag, dev_err));
 }
 
-template <int D, bool SPLIT>
+template <int D, bool QS>
 struct FlashLayout {
   static constexpr int ND = D / 64;
-  static constexpr int KST = SPLIT ? 1 : 2, VST = SPLIT ? 1 : 2;
+  static constexpr int KST = QS ? 1 : 2, VST = QS ? 1 : 2;
   static constexpr uint32_t QH = 0, QL = ND * 16384;
-  static constexpr uint32_t K = QL + (SPLIT ? ND * 16384 : 0), K_STAGE = ND * 8192;
+  static constexpr uint32_t K = QL + (QS ? ND * 16384 : 0), K_STAGE = ND * 8192;
   static constexpr uint32_t V = K + KST * K_STAGE, V_STAGE = D * 128;
   static constexpr uint32_t TILES = V + VST * V_STAGE;
   // O staging [128][D + 4] fp32 at the end, over Q, K and V
@@ -158,9 +159,9 @@ struct FlashLayout {
   static_assert(BYTES <= 113 * 1024, "two CTAs per SM");
 };
 
-template <bool E4M3, int D, bool SPLIT>
+template <bool E4M3, int D, bool QS, bool PS>
 __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args a) {
-  using L = FlashLayout<D, SPLIT>;
+  using L = FlashLayout<D, QS>;
   extern __shared__ __align__(1024) uint8_t smem[];
   float *ks_s = reinterpret_cast<float *>(smem + L::SCALES), *vs_s = ks_s + FL_SLOTS * 64;
   float *vf_s = reinterpret_cast<float *>(smem + L::VF), *vref_s = reinterpret_cast<float *>(smem + L::VREF);
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
       const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
       const uint32_t at = (uint32_t)(d >> 6) * 16384u + sw128(rr, d & 63);
       *reinterpret_cast<uint2 *>(smem + L::QH + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
-      if (SPLIT) {
+      if (QS) {
         const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
         *reinterpret_cast<uint2 *>(smem + L::QL + at) =
             make_uint2(h2_as_u32(__floats2half2_rn(x.x - g0.x, x.y - g0.y)),
@@ -368,12 +369,14 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
       auto issue_s = [&](int t) {
         const uint64_t dk = sw128_kmajor_desc(sb + L::K + (t % L::KST) * L::K_STAGE);
         const uint32_t ts = tmem + (uint32_t)(t & 1) * 64u;
+        // the lower terms first: fewer additions to a sum of full size
 #pragma unroll
-        for (int kk = 0; kk < D / 16; kk++) {
-          const uint64_t oq = ((kk >> 2) * 16384u + (kk & 3) * 32u) >> 4, ok = ((kk >> 2) * 8192u + (kk & 3) * 32u) >> 4;
-          if (SPLIT) umma_f16(ts, d_ql + oq, dk + ok, idesc_s, kk ? 1u : 0u);
-          umma_f16(ts, d_qh + oq, dk + ok, idesc_s, SPLIT || kk ? 1u : 0u);
-        }
+        for (int part = QS ? 0 : 1; part < 2; part++)
+#pragma unroll
+          for (int kk = 0; kk < D / 16; kk++) {
+            const uint64_t oq = ((kk >> 2) * 16384u + (kk & 3) * 32u) >> 4, ok = ((kk >> 2) * 8192u + (kk & 3) * 32u) >> 4;
+            umma_f16(ts, (part ? d_qh : d_ql) + oq, dk + ok, idesc_s, (QS && part) || kk ? 1u : 0u);
+          }
         umma_commit(s_full + (t & 1));
         umma_commit(k_empty + t % L::KST);
       };
@@ -401,11 +404,11 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         const uint64_t dv = sw128_kmajor_desc(sb + L::V + (t % L::VST) * L::V_STAGE);
         const uint32_t tp = tmem + (uint32_t)(t & 1) * 64u;
 #pragma unroll
-        for (int kk = 0; kk < FL_TILE / 16; kk++) {
-          const uint64_t ov = (kk * 32u) >> 4;
-          if (SPLIT) umma_f16_ts(tmem + L::T_O, tp + 32u + 8u * kk, dv + ov, idesc_o, t || kk ? 1u : 0u);
-          umma_f16_ts(tmem + L::T_O, tp + 8u * kk, dv + ov, idesc_o, SPLIT || t || kk ? 1u : 0u);
-        }
+        for (int part = PS ? 0 : 1; part < 2; part++)
+#pragma unroll
+          for (int kk = 0; kk < FL_TILE / 16; kk++)
+            umma_f16_ts(tmem + L::T_O, tp + (part ? 0u : 32u) + 8u * kk, dv + ((kk * 32u) >> 4), idesc_o,
+                        t || (PS && part) || kk ? 1u : 0u);
         umma_commit(v_empty + t % L::VST);
         umma_commit(o_done);
         // A barrier of its own for the last one: a waiter that has not seen the
@@ -514,7 +517,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
       }
       const ulonglong2 *vp = reinterpret_cast<const ulonglong2 *>(vs_s + sl * 64);
       const f32x2 rf2 = pack2(rf, rf), mr2 = pack2(-mref, -mref);
-      uint32_t ph[32], pl[SPLIT ? 32 : 1];
+      uint32_t ph[32], pl[PS ? 32 : 1];
       f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < FL_TILE / 4; c++) {
@@ -529,9 +532,9 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           unpack2(mul2(p, k ? v4.y : v4.x), w0, w1);
           const __half2 h = __floats2half2_rn(w0, w1);
           ph[2 * c + k] = h2_as_u32(h);
-          if (SPLIT) {
+          if (PS) {
             const float2 g = __half22float2(h);
-            pl[SPLIT ? 2 * c + k : 0] = h2_as_u32(__floats2half2_rn(w0 - g.x, w1 - g.y));
+            pl[PS ? 2 * c + k : 0] = h2_as_u32(__floats2half2_rn(w0 - g.x, w1 - g.y));
           }
         }
       }
@@ -543,7 +546,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           const uint32_t w = c < 16 ? s0 : s1;
           const uint32_t keep = (w >> (2 * c & 31) & 1 ? 0xffffu : 0u) | (w >> (2 * c + 1 & 31) & 1 ? 0xffff0000u : 0u);
           ph[c] &= keep;
-          if (SPLIT) pl[SPLIT ? c : 0] &= keep;
+          if (PS) pl[PS ? c : 0] &= keep;
         }
       }
       {
@@ -553,7 +556,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         l += (a0 + a1) + (b0 + b1);
       }
       tmem_st32(ts, ph);
-      if constexpr (SPLIT) tmem_st32(ts + 32u, pl);
+      if constexpr (PS) tmem_st32(ts + 32u, pl);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(p_full + (t & 1));  // two: a warp may be a tile ahead of another (S_{t+1} is there early)
@@ -648,10 +651,10 @@ void require_regs_once() {
               "GroupQueryAttention (8-bit cache): the flash kernel was built with another register count");
 }
 
-template <bool E4M3, int D, bool SPLIT>
+template <bool E4M3, int D, bool QS, bool PS>
 void launch(const Kv8Args &a, cudaStream_t s) {
-  using L = FlashLayout<D, SPLIT>;
-  constexpr auto kern = kv8_flash_kernel<E4M3, D, SPLIT>;
+  using L = FlashLayout<D, QS>;
+  constexpr auto kern = kv8_flash_kernel<E4M3, D, QS, PS>;
   set_smem_limit_once<kern>((int)L::BYTES);
   require_regs_once<kern>();
   const int nrows = a.S * (a.H / a.KVH), tiles = (nrows + FL_ROWS - 1) / FL_ROWS;
@@ -676,9 +679,9 @@ void launch(const Kv8Args &a, cudaStream_t s) {
 template <bool E4M3, int D>
 void launch_out(const Kv8Args &a, cudaStream_t s) {
   if (a.out)
-    launch<E4M3, D, true>(a, s);
+    launch<E4M3, D, true, true>(a, s);
   else
-    launch<E4M3, D, false>(a, s);
+    launch<E4M3, D, false, true>(a, s);
 }
 
 }  // namespace

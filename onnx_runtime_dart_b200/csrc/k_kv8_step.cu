@@ -8,8 +8,10 @@
 //   S^T[16 keys][8 rows] = K . Q^T,   O^T[D][8 rows] += V^T . P^T.
 // The codes are the A operands: int8 and e4m3 codes are f16 numbers exactly, so
 // they are expanded in registers and the scales applied in fp32, K's to the
-// scores and V's to the weights. Q and the weights are split into two f16 terms
-// (22 bits), so the products carry fp32 accuracy. Which D index or key an MMA
+// scores and V's to the weights. Q and (PS: fp32 rows are wanted) the weights are
+// split into two f16 terms (22 bits), so the products carry fp32 accuracy; for an
+// f16 output alone the weights are rounded to f16 once, an error like that of the
+// output's own rounding. Which D index or key an MMA
 // lane holds is free as long as both operands agree: lanes are given 16
 // consecutive bytes of a row, so no data is shuffled on its way to the tensor
 // cores; only P^T is transposed between the two products (movmatrix).
@@ -90,7 +92,7 @@ struct StepSmem {
   static_assert(ST_WARPS * R * D * 4 <= QF, "O staging fits the ring");
 };
 
-template <bool E4M3, int D, int NT>
+template <bool E4M3, int D, int NT, bool PS>
 __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, const int fused_append) {
   using L = StepShape<D>;
   using M = StepSmem<D, NT>;
@@ -211,14 +213,20 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
       if (k >= ahead) issue(warp + k * ST_WARPS, k);
   }
 
-  float o[NT][L::MT][4];
+  // With PS the products of the lower terms have sums of their own: the tensor
+  // cores cut off what an addition to a sum leaves below it, always toward zero,
+  // and half as many additions to the large sums halve that.
+  float o[NT][L::MT][4], ol[PS ? NT : 1][PS ? L::MT : 1][4];
   float m[NT][2], mref[NT][2], l[NT][2], rf[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
     for (int k = 0; k < L::MT; k++)
 #pragma unroll
-      for (int u = 0; u < 4; u++) o[nt][k][u] = 0.f;
+      for (int u = 0; u < 4; u++) {
+        o[nt][k][u] = 0.f;
+        if (PS) ol[PS ? nt : 0][PS ? k : 0][u] = 0.f;
+      }
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       m[nt][u] = -INFINITY;
@@ -339,6 +347,10 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
           for (int k = 0; k < L::MT; k++) {
             o[nt][k][u] *= fo;
             o[nt][k][2 + u] *= fo;
+            if (PS) {
+              ol[PS ? nt : 0][PS ? k : 0][u] *= fo;
+              ol[PS ? nt : 0][PS ? k : 0][2 + u] *= fo;
+            }
           }
         }
     }
@@ -358,9 +370,11 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
           w[u] = ok ? p * (k ? v1 : v0) : 0.f;  // a hidden key's scale may be NaN
         }
         const __half2 h = __floats2half2_rn(w[0], w[1]);
-        const float2 hf = __half22float2(h);
         bh[nt][k] = transpose8x8(b2m::h2_as_u32(h));
-        bl[nt][k] = transpose8x8(b2m::h2_as_u32(__floats2half2_rn(w[0] - hf.x, w[1] - hf.y)));
+        if (PS) {
+          const float2 hf = __half22float2(h);
+          bl[nt][k] = transpose8x8(b2m::h2_as_u32(__floats2half2_rn(w[0] - hf.x, w[1] - hf.y)));
+        }
       }
     // O^T += V^T . P^T
 #pragma unroll
@@ -389,10 +403,13 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
         for (int hf = 0; hf < 2; hf++)
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) mma(o[nt][(cc * L::VW + w) * 2 + hf], A[hf], bh[nt][0], bh[nt][1]);
+        if (PS) {
 #pragma unroll
-        for (int hf = 0; hf < 2; hf++)
+          for (int hf = 0; hf < 2; hf++)
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) mma(o[nt][(cc * L::VW + w) * 2 + hf], A[hf], bl[nt][0], bl[nt][1]);
+            for (int nt = 0; nt < NT; nt++)
+              mma(ol[PS ? nt : 0][PS ? (cc * L::VW + w) * 2 + hf : 0], A[hf], bl[nt][0], bl[nt][1]);
+        }
       }
     }
     slot = slot + 1 == ST_STAGES ? 0 : slot + 1;
@@ -400,6 +417,15 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
   }
   cp_wait<0>();
   __syncthreads();  // the rings are drained: the states reuse them
+
+  if (PS) {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int k = 0; k < L::MT; k++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) o[nt][k][u] += ol[PS ? nt : 0][PS ? k : 0][u];
+  }
 
   // Warp states: m, l per row and O (in the values' own scale).
   float *so = reinterpret_cast<float *>(smem);
@@ -482,10 +508,10 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
   if (CL > 1) cluster.sync();  // the others have read this CTA's state
 }
 
-template <bool E4M3, int D, int NT>
+template <bool E4M3, int D, int NT, bool PS>
 void launch(const Kv8Args &a, cudaStream_t s) {
   using M = StepSmem<D, NT>;
-  constexpr auto kern = kv8_step_kernel<E4M3, D, NT>;
+  constexpr auto kern = kv8_step_kernel<E4M3, D, NT, PS>;
   b2m::set_smem_limit_once<kern>(M::BYTES);
   const int nrows = a.S * (a.H / a.KVH), tiles = (nrows + M::R - 1) / M::R;
   // One new row per sequence is appended beside the query rows; more would hold up
@@ -519,12 +545,20 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   B2M_CUDA(cudaLaunchKernelEx(&cfg, kern, a, fused ? 1 : 0));
 }
 
+template <bool E4M3, int D, int NT>
+void launch_out(const Kv8Args &a, cudaStream_t s) {
+  if (a.out)
+    launch<E4M3, D, NT, true>(a, s);
+  else
+    launch<E4M3, D, NT, false>(a, s);
+}
+
 template <bool E4M3, int D>
 void launch_rows(const Kv8Args &a, cudaStream_t s) {
   if (a.S * (a.H / a.KVH) <= 8)
-    launch<E4M3, D, 1>(a, s);
+    launch_out<E4M3, D, 1>(a, s);
   else
-    launch<E4M3, D, 2>(a, s);
+    launch_out<E4M3, D, 2>(a, s);
 }
 
 template <bool E4M3>
@@ -534,7 +568,7 @@ void launch_dim(const Kv8Args &a, cudaStream_t s) {
     case 64: return launch_rows<E4M3, 64>(a, s);
     case 96: return launch_rows<E4M3, 96>(a, s);
     case 128: return launch_rows<E4M3, 128>(a, s);
-    default: return launch<E4M3, 256, 1>(a, s);
+    default: return launch_out<E4M3, 256, 1>(a, s);
   }
 }
 
