@@ -26,16 +26,18 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const Kv8Args a) {
   append_row(a, b, i, kvh, side, a.past[b], stage[warp], lane);
 }
 
-// The same for rows of whole float4s: one warp per (token, kv head), both sides.
+// The same for rows of whole float4s: half a warp per (token, kv head), both
+// sides. Bound by issue slots, not by memory (8 D bytes in, 2 D + 8 out): what a
+// row costs beside its elements (the norm factor, the maximum in double) is paid
+// once for two rows.
 template <bool E4M3, int NCH>
-__global__ void __launch_bounds__(256) kv8_append_vec_kernel(const Kv8Args a) {
+__global__ void __launch_bounds__(256, NCH == 4 ? 1 : 3) kv8_append_vec_kernel(const Kv8Args a) {
   pdl_launch_dependents();
-  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned item = blockIdx.x * 8 + warp;  // (token, kv head): the launcher keeps it below 2^31
+  const unsigned item = blockIdx.x * 16 + (threadIdx.x >> 4);  // (token, kv head): the launcher keeps it below 2^31
+  if ((item & ~1u) >= (unsigned)a.S * (unsigned)a.KVH) return;  // the whole warp
   const unsigned i = item / (unsigned)a.KVH;
-  if (i >= (unsigned)a.S) return;
   const int b = blockIdx.y;
-  append_pair_vec<E4M3, NCH>(a, b, (int)i, (int)(item - i * a.KVH), a.past[b], (int)lane);
+  append_vec<E4M3, 16, NCH>(a, b, (int)i, (int)(item - i * a.KVH), 3, a.past[b], i < (unsigned)a.S);
 }
 
 // The values of n cached positions from start[b] (or 0) on, [B][KVH][n][D]
@@ -55,6 +57,36 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Args a, const in
     return;
   }
   const int64_t row = bk * a.CAP + pos;
+  // Four codes a lane where both ends allow it, all loads ahead of the stores.
+  auto al16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  if ((a.D & 3) == 0 && al16(k_out) && al16(v_out)) {
+    uint32_t w[2][2];
+    float s[2];
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
+      if (!(side ? v_out : k_out)) continue;
+      s[side] = (side ? a.vs : a.ks)[row];
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+        if (4 * (lane + 32 * u) < a.D)
+          w[side][u] = reinterpret_cast<const uint32_t *>((side ? a.vc : a.kc) + row * a.D)[lane + 32 * u];
+    }
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
+      float *out = side ? v_out : k_out;
+      if (!out) continue;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+        if (4 * (lane + 32 * u) < a.D) {
+          const uint32_t c = w[side][u];
+          float4 v;
+          v.x = code_value<E4M3>((uint8_t)c) * s[side], v.y = code_value<E4M3>((uint8_t)(c >> 8)) * s[side];
+          v.z = code_value<E4M3>((uint8_t)(c >> 16)) * s[side], v.w = code_value<E4M3>((uint8_t)(c >> 24)) * s[side];
+          reinterpret_cast<float4 *>(out + item * a.D)[lane + 32 * u] = v;
+        }
+    }
+    return;
+  }
 #pragma unroll
   for (int side = 0; side < 2; side++) {
     float *out = side ? v_out : k_out;
@@ -233,18 +265,11 @@ void launch_kv8_append(const Kv8Args &a, cudaStream_t s) {
   const int64_t items = (int64_t)a.B * a.S * a.KVH * 2;
   if (items == 0) return;
   if (append_rows_vec(a) && (int64_t)a.S * a.KVH < ((int64_t)1 << 31) && a.B <= 65535) {
-    const dim3 grid((unsigned)(((int64_t)a.S * a.KVH + 7) / 8), (unsigned)a.B);
-    if (a.D <= 128) {
-      if (a.e4m3)
-        kv8_append_vec_kernel<true, 1><<<grid, 256, 0, s>>>(a);
-      else
-        kv8_append_vec_kernel<false, 1><<<grid, 256, 0, s>>>(a);
-    } else {
-      if (a.e4m3)
-        kv8_append_vec_kernel<true, 2><<<grid, 256, 0, s>>>(a);
-      else
-        kv8_append_vec_kernel<false, 2><<<grid, 256, 0, s>>>(a);
-    }
+    const dim3 grid((unsigned)(((int64_t)a.S * a.KVH + 15) / 16), (unsigned)a.B);
+    auto kern = a.D <= 64 ? (a.e4m3 ? kv8_append_vec_kernel<true, 1> : kv8_append_vec_kernel<false, 1>)
+                : a.D <= 128 ? (a.e4m3 ? kv8_append_vec_kernel<true, 2> : kv8_append_vec_kernel<false, 2>)
+                             : (a.e4m3 ? kv8_append_vec_kernel<true, 4> : kv8_append_vec_kernel<false, 4>);
+    kern<<<grid, 256, 0, s>>>(a);
     B2M_CUDA(cudaGetLastError());
     return;
   }

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
 #pragma unroll 1
     for (int it = warp; it < nnew + R / 4; it += ST_WARPS) {
       if (it < nnew) {
-        append_side_vec<E4M3, (D + 127) / 128>(a, b, i0 + (it >> 1), kvh, it & 1, a.past[b], lane);
+        append_vec<E4M3, 32, (D + 127) / 128>(a, b, i0 + (it >> 1), kvh, 1 << (it & 1), a.past[b], true);
       } else {
         const int rr = 4 * (it - nnew) + (lane >> 3);
         QRow<D> q;

@@ -160,6 +160,13 @@ struct RowChunk {
   float c[4], sn[4];   // x_rot = x c - w sn (the sign of the second half is in sn)
 };
 
+// max(|a|, |b|, |c|), NaN if one is.
+__device__ __forceinline__ float max3_nan_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
+}
+
 template <bool NORM, bool ROT>
 __device__ __forceinline__ double chunk_exact(const RowChunk &r, int k, double inv, bool turn) {
   const double x = NORM ? (double)r.x[k] * inv * r.g[k] : (double)r.x[k];
@@ -173,11 +180,37 @@ __device__ __forceinline__ uint32_t exact_code(double x, float s, bool e4m3) {
   return e4m3 ? e4m3_code(t) : (uint32_t)(uint8_t)(int8_t)(int)rint(t);
 }
 
-// NCH chunks of four values per lane: values 4 (lane + 32 i) .. + 3 of the row.
+// Reductions over the LPR lanes (32, or either half of a warp) of a row; the whole
+// warp takes part.
+template <int LPR>
+__device__ __forceinline__ double row_sum_d(double v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int LPR>
+__device__ __forceinline__ double row_max_d(double v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+template <int LPR>
+__device__ __forceinline__ uint32_t row_max_u(uint32_t v) {
+  if constexpr (LPR == 32) {
+    return __reduce_max_sync(0xffffffffu, v);
+  } else {
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  }
+}
+
+// NCH chunks of four values per lane, LPR lanes per row: lane l of the row holds
+// values 4 (l + LPR i) .. + 3. Writes nothing where !ok.
 // NORM: the head norm comes first; ROT: the chunks that `turn` marks are rotated.
-template <bool E4M3, int NCH, bool NORM, bool ROT>
+template <bool E4M3, int LPR, int NCH, bool NORM, bool ROT>
 __device__ __forceinline__ void quantise_chunks(RowChunk (&r)[NCH], int D, double eps, const bool (&turn)[NCH],
-                                                uint8_t *codes, float *scale, int lane) {
+                                                uint8_t *codes, float *scale, int l, bool ok) {
   constexpr bool real = NORM || ROT;  // x is more than its fp32 value
   constexpr float top = E4M3 ? 448.f : 127.f;
   double inv = 1.0;
@@ -188,7 +221,7 @@ __device__ __forceinline__ void quantise_chunks(RowChunk (&r)[NCH], int D, doubl
     for (int i = 0; i < NCH; i++)
 #pragma unroll
       for (int k = 0; k < 4; k++) ss = fma((double)r[i].x[k], (double)r[i].x[k], ss);
-    const double v = warp_sum_d(ss) / D + eps;
+    const double v = row_sum_d<LPR>(ss) / D + eps;
     // 1 / sqrt(v): two Newton steps from the fp32 value (relative error 2^-50);
     // outside fp32's comfortable range by the library
     if (v > 1e-30 && v < 1e30) {
@@ -201,8 +234,7 @@ __device__ __forceinline__ void quantise_chunks(RowChunk (&r)[NCH], int D, doubl
     invf = (float)inv;
   }
   float x[NCH][4];
-  uint32_t mx = 0;
-  float mag = 0.f;  // largest sum of the magnitudes that make up a value
+  float top_x = 0.f, mag = 0.f;  // largest value; largest sum of the magnitudes that make up one
 #pragma unroll
   for (int i = 0; i < NCH; i++) {
 #pragma unroll
@@ -217,49 +249,55 @@ __device__ __forceinline__ void quantise_chunks(RowChunk (&r)[NCH], int D, doubl
         mag = fmaxf(mag, fabsf(v));
       }
       x[i][k] = v;
-      mx = max(mx, __float_as_uint(v) & 0x7fffffffu);  // infinities and NaN order above
     }
+    top_x = max3_nan_abs(top_x, x[i][0], x[i][1]);
+    top_x = max3_nan_abs(top_x, x[i][2], x[i][3]);
   }
-  mx = __reduce_max_sync(0xffffffffu, mx);
+  const uint32_t mx = row_max_u<LPR>(__float_as_uint(top_x));  // infinities and NaN order above
   const float amaxf = __uint_as_float(mx);
   // |fp32 x - x|: at most seven roundings of 2^-24 of mag
-  const float xerr = real ? __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mag))) * 0x1p-20f : 0.f;
+  const float xerr = real ? __uint_as_float(row_max_u<LPR>(__float_as_uint(mag))) * 0x1p-20f : 0.f;
   float s;
-  if (mx >= 0x7f800000u) {
-    s = __int_as_float(0x7fc00000);
-    // (an infinity that only the fp32 arithmetic made is told apart below)
-  } else if (!real) {
+  if (!real) {
     // amaxf / top, rounded once: Markstein's quotient by the rounded reciprocal
-    const float q = amaxf * (1.f / top);
-    s = fmaf(fmaf(-q, top, amaxf), 1.f / top, q);
+    const float t = amaxf * (1.f / top);
+    s = fmaf(fmaf(-t, top, amaxf), 1.f / top, t);
   } else {
     double am = 0.0;
     const float near = amaxf - 2.f * xerr;
+    if (fabsf(top_x) >= near) {  // few lanes hold a candidate
 #pragma unroll
-    for (int i = 0; i < NCH; i++)
+      for (int i = 0; i < NCH; i++)
 #pragma unroll
-      for (int k = 0; k < 4; k++)
-        if (fabsf(x[i][k]) >= near) am = fmax(am, fabs(chunk_exact<NORM, ROT>(r[i], k, inv, turn[i])));
-    const unsigned cand = __ballot_sync(0xffffffffu, am > 0.0);  // one lane as a rule
-    am = (cand & (cand - 1)) == 0 ? __shfl_sync(0xffffffffu, am, cand ? __ffs(cand) - 1 : 0) : warp_max_d(am);
+        for (int k = 0; k < 4; k++)
+          if (fabsf(x[i][k]) >= near) am = fmax(am, fabs(chunk_exact<NORM, ROT>(r[i], k, inv, turn[i])));
+    }
+    // one lane of the row as a rule
+    const unsigned half = LPR == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+    const unsigned cand = __ballot_sync(0xffffffffu, am > 0.0) & half;
+    if (__any_sync(0xffffffffu, (cand & (cand - 1)) != 0))
+      am = row_max_d<LPR>(am);
+    else
+      am = __shfl_sync(0xffffffffu, am, cand ? __ffs(cand) - 1 : 0);
     s = (float)(am * (1.0 / (double)top));
   }
   // Values near the ends of fp32's range: everything in double.
   const bool slow_row = real ? !(amaxf > 1e-25f && amaxf < 1e30f) : !(amaxf > 1e-30f && mx < 0x7f800000u);
   uint32_t word[NCH];
-  if (slow_row) {
+  if (__any_sync(0xffffffffu, slow_row)) {  // (both rows of a warp: the exact way is right for either)
     double am = 0.0;
-    bool bad = false;
+    uint32_t bad = 0;
 #pragma unroll
     for (int i = 0; i < NCH; i++)
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const double v = chunk_exact<NORM, ROT>(r[i], k, inv, turn[i]);
-        bad |= !isfinite(v);
+        bad |= isfinite(v) ? 0u : 1u;
         am = fmax(am, fabs(v));
       }
-    bad = __any_sync(0xffffffffu, bad);
-    s = bad ? __int_as_float(0x7fc00000) : (float)(warp_max_d(am) / (double)top);
+    bad = row_max_u<LPR>(bad);
+    am = row_max_d<LPR>(am);
+    s = bad ? __int_as_float(0x7fc00000) : (float)(am / (double)top);
 #pragma unroll
     for (int i = 0; i < NCH; i++) {
       word[i] = 0;
@@ -270,47 +308,46 @@ __device__ __forceinline__ void quantise_chunks(RowChunk (&r)[NCH], int D, doubl
   } else {
     const float is = __fdividef(1.f, s);  // (its error of some 2^-23 is within the 2^-20 below)
     const float wabs = xerr * is;  // |t - x / s| is at most this and 2^-20 of t
-    uint32_t doubt = 0;
+    uint32_t doubt[NCH], any = 0;  // bytes whose code depends on the error
 #pragma unroll
     for (int i = 0; i < NCH; i++) {
-      uint32_t c[4];
+      uint32_t lo[4], hi[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const float t = x[i][k] * is, w = fmaf(fabsf(t), 0x1p-20f, wabs);
         if (E4M3) {
-          const uint32_t p = __nv_cvt_float2_to_fp8x2(make_float2(t - w, t + w), __NV_SATFINITE, __NV_E4M3);
-          c[k] = p;
-          doubt |= ((p ^ (p >> 8)) & 0xffu) ? 1u << (4 * i + k) : 0u;
+          lo[k] = __nv_cvt_float2_to_fp8x2(make_float2(t - w, t + w), __NV_SATFINITE, __NV_E4M3);
         } else {
-          const uint32_t lo = __float_as_uint((t - w) + 12582912.f), hi = __float_as_uint((t + w) + 12582912.f);
-          c[k] = lo;
-          doubt |= lo != hi ? 1u << (4 * i + k) : 0u;
+          lo[k] = __float_as_uint((t - w) + 12582912.f);
+          hi[k] = __float_as_uint((t + w) + 12582912.f);
         }
       }
-      word[i] = b2m::prmt(b2m::prmt(c[0], c[1], 0x0040), b2m::prmt(c[2], c[3], 0x0040), 0x5410);
+      if (E4M3) {
+        const uint32_t u = b2m::prmt(lo[0], lo[1], 0x5410), v = b2m::prmt(lo[2], lo[3], 0x5410);  // pairs (lo, hi)
+        word[i] = b2m::prmt(u, v, 0x6420);
+        doubt[i] = word[i] ^ b2m::prmt(u, v, 0x7531);
+      } else {
+        word[i] = b2m::prmt(b2m::prmt(lo[0], lo[1], 0x0040), b2m::prmt(lo[2], lo[3], 0x0040), 0x5410);
+        doubt[i] = word[i] ^ b2m::prmt(b2m::prmt(hi[0], hi[1], 0x0040), b2m::prmt(hi[2], hi[3], 0x0040), 0x5410);
+      }
+      any |= doubt[i];
     }
-    if (doubt) {
+    if (any) {
 #pragma unroll
       for (int i = 0; i < NCH; i++)
-#pragma unroll 1
-        for (int k = 0; k < 4; k++) {
-          if (!(doubt >> (4 * i + k) & 1)) continue;
-          RowChunk e;  // (selected by hand: k is not a constant here)
 #pragma unroll
-          for (int u = 0; u < 4; u++)
-            if (u == k) {
-              e.x[0] = r[i].x[u], e.w[0] = r[i].w[u], e.g[0] = r[i].g[u];
-              e.gw[0] = r[i].gw[u], e.c[0] = r[i].c[u], e.sn[0] = r[i].sn[u];
-            }
-          const uint32_t code = exact_code(chunk_exact<NORM, ROT>(e, 0, inv, turn[i]), s, E4M3);
-          word[i] = (word[i] & ~(0xffu << (8 * k))) | (code << (8 * k));
-        }
+        for (int k = 0; k < 4; k++)
+          if (doubt[i] >> (8 * k) & 0xffu) {
+            const uint32_t code = exact_code(chunk_exact<NORM, ROT>(r[i], k, inv, turn[i]), s, E4M3);
+            word[i] = (word[i] & ~(0xffu << (8 * k))) | (code << (8 * k));
+          }
     }
   }
-  if (lane == 0) *scale = s;
+  if (!ok) return;
+  if (l == 0) *scale = s;
 #pragma unroll
   for (int i = 0; i < NCH; i++)
-    if (4 * (lane + 32 * i) < D) *reinterpret_cast<uint32_t *>(codes + 4 * (lane + 32 * i)) = word[i];
+    if (4 * (l + LPR * i) < D) *reinterpret_cast<uint32_t *>(codes + 4 * (l + LPR * i)) = word[i];
 }
 
 // The rows quantise_chunks takes.
@@ -320,13 +357,13 @@ inline bool append_rows_vec(const Kv8Args &a) {
          (!a.cos || (a.rot % 8 == 0 && a.half % 4 == 0 && al(a.cos) && al(a.sin)));
 }
 
-// Loads one side's row of new token i (position pos for the rotary).
-template <int NCH>
+// Loads one side's row of a new token (position pos for the rotary).
+template <int LPR, int NCH>
 __device__ __forceinline__ void load_chunks(const Kv8Args &a, const float *src, const float *gain, const float *cos,
-                                            int64_t pos, RowChunk (&r)[NCH], bool (&turn)[NCH], int lane) {
+                                            int64_t pos, RowChunk (&r)[NCH], bool (&turn)[NCH], int l) {
 #pragma unroll
   for (int i = 0; i < NCH; i++) {
-    const int d = 4 * (lane + 32 * i);
+    const int d = 4 * (l + LPR * i);
     turn[i] = false;
     auto put = [](float *dst, const float *p) {
       const float4 v = *reinterpret_cast<const float4 *>(p);
@@ -365,64 +402,47 @@ __device__ __forceinline__ void load_chunks(const Kv8Args &a, const float *src, 
   }
 }
 
-// append_row for rows that append_rows_vec accepts: both sides of new token i.
-template <bool E4M3, int NCH>
-__device__ __forceinline__ void append_pair_vec(const Kv8Args &a, int b, int i, int kvh, int past, int lane) {
-  const int64_t pos = token_pos(a, b, i, past);
-  if (past < 0 || (a.cos && pos < 0)) {
-    if (lane == 0 && a.err) b2m::set_dev_error(a.err, B2M_DEVERR_INDEX);
-    return;
-  }
-  if ((int64_t)past + i >= a.CAP) {
-    if (lane == 0 && a.err) b2m::set_dev_error(a.err, B2M_DEVERR_CACHE_FULL);
-    return;
-  }
-  const int64_t off = ((int64_t)b * a.S + i) * a.kv_rs + (int64_t)kvh * a.D;
-  const int64_t row = ((int64_t)b * a.KVH + kvh) * a.CAP + past + i;
-  const float *gain = a.k_gain ? a.k_gain + (int64_t)kvh * a.D : nullptr;
-  RowChunk rk[NCH], rv[NCH];
-  bool tk[NCH], tv[NCH];
-  load_chunks<NCH>(a, a.v + off, nullptr, nullptr, 0, rv, tv, lane);
-  load_chunks<NCH>(a, a.k + off, gain, pos >= a.CAP ? nullptr : a.cos, pos, rk, tk, lane);
-  quantise_chunks<E4M3, NCH, false, false>(rv, a.D, 0.0, tv, a.vc + row * a.D, a.vs + row, lane);
-  if (gain)  // (ROT without a table: no chunk is marked)
-    quantise_chunks<E4M3, NCH, true, true>(rk, a.D, a.eps, tk, a.kc + row * a.D, a.ks + row, lane);
-  else if (a.cos)
-    quantise_chunks<E4M3, NCH, false, true>(rk, a.D, 0.0, tk, a.kc + row * a.D, a.ks + row, lane);
-  else
-    quantise_chunks<E4M3, NCH, false, false>(rk, a.D, 0.0, tk, a.kc + row * a.D, a.ks + row, lane);
+// Where a new token's row goes; false (and the device error) where it is refused.
+struct NewRow {
+  int64_t pos, off, row;
+  const float *gain, *cos;
+};
+__device__ __forceinline__ bool place_row(const Kv8Args &a, int b, int i, int kvh, int past, NewRow &w) {
+  w.pos = token_pos(a, b, i, past);
+  const bool index = past < 0 || (a.cos && w.pos < 0), full = (int64_t)past + i >= a.CAP;
+  if ((index || full) && a.err) b2m::set_dev_error(a.err, index ? B2M_DEVERR_INDEX : B2M_DEVERR_CACHE_FULL);
+  w.off = ((int64_t)b * a.S + i) * a.kv_rs + (int64_t)kvh * a.D;
+  w.row = ((int64_t)b * a.KVH + kvh) * a.CAP + past + i;
+  w.gain = a.k_gain ? a.k_gain + (int64_t)kvh * a.D : nullptr;
+  w.cos = w.pos < 0 || w.pos >= a.CAP ? nullptr : a.cos;  // the table's positions
+  return !index && !full;
 }
 
-// One side of append_pair_vec.
-template <bool E4M3, int NCH>
-__device__ __forceinline__ void append_side_vec(const Kv8Args &a, int b, int i, int kvh, int side, int past, int lane) {
-  const int64_t pos = token_pos(a, b, i, past);
-  if (past < 0 || (a.cos && pos < 0)) {
-    if (lane == 0 && a.err) b2m::set_dev_error(a.err, B2M_DEVERR_INDEX);
-    return;
+// append_row for rows that append_rows_vec accepts: the sides of `sides` (bit 0:
+// the key, bit 1: the value) of one new token's kv head per LPR lanes, all loads
+// ahead of the arithmetic. All 32 lanes call it, `ok` false where there is none.
+template <bool E4M3, int LPR, int NCH>
+__device__ __forceinline__ void append_vec(const Kv8Args &a, int b, int i, int kvh, int sides, int past, bool ok) {
+  const int l = threadIdx.x & (LPR - 1);
+  NewRow w;
+  ok = ok && place_row(a, b, i, kvh, past, w);
+  if (!ok) w.off = 0, w.row = 0, w.pos = 0, w.gain = nullptr, w.cos = nullptr;  // (reads the first row, writes nothing)
+  RowChunk rk[NCH], rv[NCH];
+  bool tk[NCH], tv[NCH];
+  if (sides & 2) load_chunks<LPR, NCH>(a, a.v + w.off, nullptr, nullptr, 0, rv, tv, l);
+  if (sides & 1) load_chunks<LPR, NCH>(a, a.k + w.off, w.gain, w.cos, w.pos, rk, tk, l);
+  if (sides & 2)
+    quantise_chunks<E4M3, LPR, NCH, false, false>(rv, a.D, 0.0, tv, a.vc + w.row * a.D, a.vs + w.row, l, ok);
+  if (sides & 1) {
+    uint8_t *codes = a.kc + w.row * a.D;
+    float *scale = a.ks + w.row;
+    if (a.k_gain)  // (ROT without a table: no chunk is marked)
+      quantise_chunks<E4M3, LPR, NCH, true, true>(rk, a.D, a.eps, tk, codes, scale, l, ok);
+    else if (a.cos)
+      quantise_chunks<E4M3, LPR, NCH, false, true>(rk, a.D, 0.0, tk, codes, scale, l, ok);
+    else
+      quantise_chunks<E4M3, LPR, NCH, false, false>(rk, a.D, 0.0, tk, codes, scale, l, ok);
   }
-  if ((int64_t)past + i >= a.CAP) {
-    if (lane == 0 && a.err) b2m::set_dev_error(a.err, B2M_DEVERR_CACHE_FULL);
-    return;
-  }
-  const int64_t off = ((int64_t)b * a.S + i) * a.kv_rs + (int64_t)kvh * a.D;
-  const int64_t row = ((int64_t)b * a.KVH + kvh) * a.CAP + past + i;
-  const float *gain = a.k_gain ? a.k_gain + (int64_t)kvh * a.D : nullptr;
-  const float *cos = pos >= a.CAP ? nullptr : a.cos;  // the table's positions
-  RowChunk r[NCH];
-  bool turn[NCH];
-  if (side) {
-    load_chunks<NCH>(a, a.v + off, nullptr, nullptr, 0, r, turn, lane);
-    quantise_chunks<E4M3, NCH, false, false>(r, a.D, 0.0, turn, a.vc + row * a.D, a.vs + row, lane);
-    return;
-  }
-  load_chunks<NCH>(a, a.k + off, gain, cos, pos, r, turn, lane);
-  if (gain)  // (ROT without a table: no chunk is marked)
-    quantise_chunks<E4M3, NCH, true, true>(r, a.D, a.eps, turn, a.kc + row * a.D, a.ks + row, lane);
-  else if (a.cos)
-    quantise_chunks<E4M3, NCH, false, true>(r, a.D, 0.0, turn, a.kc + row * a.D, a.ks + row, lane);
-  else
-    quantise_chunks<E4M3, NCH, false, false>(r, a.D, 0.0, turn, a.kc + row * a.D, a.ks + row, lane);
 }
 
 // ---- query rows -------------------------------------------------------------
