@@ -610,15 +610,33 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     if (CL == 1) {
       acc = *reinterpret_cast<const float4 *>(src);
     } else {
+      // four ranks at once, their loads ahead of the first use (one after the other: 56 us for 53)
       float top = -INFINITY, sum = 0.f;
-      for (int q = 0; q < CL; q++) top = fmaxf(top, *cluster.map_shared_rank(row_m + rr, q));
-      for (int q = 0; q < CL; q++) {
-        const float sl = *cluster.map_shared_rank(row_l + rr, q), sm = *cluster.map_shared_rank(row_m + rr, q);
-        // none if that rank saw no key; with a NaN sum and no maximum the NaN is passed on
-        const float f = sl == 0.f ? 0.f : (sm == -INFINITY ? 1.f : ex2(sm - top));
-        const float4 v = *cluster.map_shared_rank(reinterpret_cast<const float4 *>(src), q);
-        sum += sl * f;
-        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+      for (int q0 = 0; q0 < CL; q0 += 4) {
+        float sm[4], sl[4];
+        const float was = top;
+        float4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int q = q0 + k;
+          sm[k] = -INFINITY, sl[k] = 0.f, v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (q < CL) {
+            sm[k] = *cluster.map_shared_rank(row_m + rr, q);
+            sl[k] = *cluster.map_shared_rank(row_l + rr, q);
+            v[k] = *cluster.map_shared_rank(reinterpret_cast<const float4 *>(src), q);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) top = fmaxf(top, sm[k]);
+        // none if a rank saw no key; with a NaN sum and no maximum the NaN is passed on
+        const float keep = sum == 0.f ? 0.f : (was == -INFINITY ? 1.f : ex2(was - top));
+        sum *= keep, acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float f = sl[k] == 0.f ? 0.f : (sm[k] == -INFINITY ? 1.f : ex2(sm[k] - top));
+          sum += sl[k] * f;
+          acc.x += v[k].x * f, acc.y += v[k].y * f, acc.z += v[k].z * f, acc.w += v[k].w * f;
+        }
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;

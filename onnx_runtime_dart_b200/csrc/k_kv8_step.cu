@@ -486,15 +486,31 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, c
     if (r >= nrows) continue;
     float top = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q = 0; q < CL; q++) top = fmaxf(top, CL > 1 ? *cluster.map_shared_rank(cm + rr, q) : cm[rr]);
-    for (int q = 0; q < CL; q++) {
-      const float sl = CL > 1 ? *cluster.map_shared_rank(cl_ + rr, q) : cl_[rr];
-      const float sm = CL > 1 ? *cluster.map_shared_rank(cm + rr, q) : cm[rr];
-      const float f = share(sm, sl, top);
-      const float4 *src = reinterpret_cast<const float4 *>(so) + e;
-      const float4 v = CL > 1 ? *cluster.map_shared_rank(src, q) : *src;
-      sum += sl * f;
-      acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+    // (eight ranks' loads at once: their latency is what this costs)
+    for (int q0 = 0; q0 < CL; q0 += 8) {
+      float sm[8], sl[8], was = top;
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int q = q0 + k;
+        sm[k] = -INFINITY, sl[k] = 0.f, v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (q < CL) {
+          const float4 *src = reinterpret_cast<const float4 *>(so) + e;
+          sm[k] = CL > 1 ? *cluster.map_shared_rank(cm + rr, q) : cm[rr];
+          sl[k] = CL > 1 ? *cluster.map_shared_rank(cl_ + rr, q) : cl_[rr];
+          v[k] = CL > 1 ? *cluster.map_shared_rank(src, q) : *src;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k++) top = fmaxf(top, sm[k]);
+      const float keep = share(was, sum, top);
+      sum *= keep, acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const float f = share(sm[k], sl[k], top);
+        sum += sl[k] * f;
+        acc.x += v[k].x * f, acc.y += v[k].y * f, acc.z += v[k].z * f, acc.w += v[k].w * f;
+      }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that saw nothing: zeros
     acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;

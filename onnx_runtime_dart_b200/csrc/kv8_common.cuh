@@ -476,8 +476,23 @@ __device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int
   const int64_t pos = token_pos(a, b, i, past);
   const bool turn = a.cos && pos >= 0 && pos < a.CAP;
   const int hr = a.rot >> 1;
+  // The whole head in halves: a chunk's partner is NC / 2 chunks on, in this lane.
+  const bool halves = turn && a.rot == D && !a.interleaved && NC % 2 == 0;
+  constexpr int NH = NC / 2 > 0 ? NC / 2 : 1;
+  float4 g4[NC], c4[NH], n4[NH];  // all loads ahead of the first use
 #pragma unroll
-  for (int u = 0; u < NC; u++) o.v[u] = *reinterpret_cast<const float4 *>(src + 4 * (l8 + 8 * u));
+  for (int u = 0; u < NC; u++) {
+    o.v[u] = *reinterpret_cast<const float4 *>(src + 4 * (l8 + 8 * u));
+    if (gain) g4[u] = *reinterpret_cast<const float4 *>(gain + 4 * (l8 + 8 * u));
+  }
+  if (halves) {
+#pragma unroll
+    for (int u = 0; u < NC / 2; u++) {
+      const int64_t at = pos * a.half + 4 * (l8 + 8 * u);
+      c4[u] = *reinterpret_cast<const float4 *>(a.cos + at);
+      n4[u] = *reinterpret_cast<const float4 *>(a.sin + at);
+    }
+  }
   float inv = 1.f;
   if (gain) {
     float ss = 0.f;
@@ -491,16 +506,13 @@ __device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int
   if (gain) {
 #pragma unroll
     for (int u = 0; u < NC; u++) {
-      const float4 g4 = *reinterpret_cast<const float4 *>(gain + 4 * (l8 + 8 * u));
-      o.v[u].x *= inv * g4.x, o.v[u].y *= inv * g4.y, o.v[u].z *= inv * g4.z, o.v[u].w *= inv * g4.w;
+      o.v[u].x *= inv * g4[u].x, o.v[u].y *= inv * g4[u].y, o.v[u].z *= inv * g4[u].z, o.v[u].w *= inv * g4[u].w;
     }
   }
-  if (turn && a.rot == D && !a.interleaved && NC % 2 == 0) {
-    // The whole head in halves: a chunk's partner is NC / 2 chunks on, in this lane.
+  if (halves) {
 #pragma unroll
     for (int u = 0; u < NC / 2; u++) {
-      const int64_t at = pos * a.half + 4 * (l8 + 8 * u);
-      const float4 c = *reinterpret_cast<const float4 *>(a.cos + at), n = *reinterpret_cast<const float4 *>(a.sin + at);
+      const float4 c = c4[u], n = n4[u];
       const float4 x = o.v[u], y = o.v[u + NC / 2];
       o.v[u] = make_float4(x.x * c.x - y.x * n.x, x.y * c.y - y.y * n.y, x.z * c.z - y.z * n.z, x.w * c.w - y.w * n.w);
       o.v[u + NC / 2] =
