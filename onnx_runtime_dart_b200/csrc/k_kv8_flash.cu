@@ -7,9 +7,10 @@
 //   warps 4-7  expand a tile's codes (exact f16 numbers) into shared memory, K as
 //              [64 keys][D], V transposed as [D][64 keys] (128-byte swizzle), the
 //              next tile's codes already in flight in registers;
-//   warp 8     (of a third warpgroup) one thread issues S_j = Q . K_j^T (S in TMEM, two buffers) and
-//              O += P_j . V_j with P in TMEM as the A operand; S_{j+1} is issued
-//              before P_j is waited for, so the tensor cores work under the softmax;
+//   warp 8     (of a third warpgroup) one thread issues S_j = Q . K_j^T (S in TMEM,
+//              two buffers) and O += P_j . V_j with P in TMEM as the A operand;
+//              S_{j+1} is issued before P_j is waited for, so the tensor cores
+//              work under the softmax;
 //   warps 0-3  a thread per query row (= TMEM lane): scores times K's scale,
 //              the causal or tree mask, exp2 against a reference that only moves
 //              when a score passes it by 2^5 (O in TMEM is rescaled then), the
@@ -25,6 +26,11 @@
 // Few row tiles over many keys (a tree on long sequences): the CTAs of a cluster
 // split the keys and merge their O, m and l through distributed shared memory in
 // rank order; no workspace, no atomics.
+//
+// 4 x 2048 causal tokens (16 heads on 8) take 245 us: 280 TFLOP/s of wanted products,
+// tensor pipe 25% busy (P's second term included), issue slots 52%. What bounds it is the
+// instructions of the softmax and of the expansion (some 4500 per 64-key tile and
+// CTA) and, per CTA, 14K cycles of query loading and 8K of output beside 75K of loop.
 //
 // Every wait is bounded; one that gives up records the device error and all
 // roles leave their loops.

@@ -16,10 +16,14 @@
 // consecutive bytes of a row, so no data is shuffled on its way to the tensor
 // cores; only P^T is transposed between the two products (movmatrix).
 //
-// Bound by HBM (2 D + 8 bytes per key of a kv head). Each lane copies the bytes
-// it will use itself into a ring of its own in shared memory (cp.async), three
-// tiles ahead, so that enough loads are in flight without registers and no
-// barrier is needed in the loop.
+// Should be bound by HBM (2 D + 8 bytes per key of a kv head): 64 sequences over
+// 4096 .. 8191 positions of 8 kv heads take 168 us, 4.98 TB/s (floor 129); the warps'
+// own chains (expand, product, exp2, product) and the part-empty last wave are the
+// rest, issue slots 49% used. Each lane copies the bytes it will use itself into a
+// ring of its own in shared memory (cp.async), two tiles ahead, so that enough
+// loads are in flight without registers and no barrier is needed in the loop (one
+// tile ahead 184 us, three 169; four CTAs per SM instead of three 184, six warps
+// per CTA 185, eight 223).
 //
 // The softmax reference m moves only when a score passes it by more than 2^5 (a
 // warp vote); weights are scaled by 2^10 so that f16 keeps small ones. V scales
@@ -38,7 +42,7 @@ namespace {
 namespace cg = cooperative_groups;
 using namespace kv8;
 
-constexpr int ST_WARPS = 4, ST_THREADS = 32 * ST_WARPS, ST_STAGES = 4;
+constexpr int ST_WARPS = 4, ST_THREADS = 32 * ST_WARPS, ST_STAGES = 3;
 constexpr float P_BIAS = 10.f, M_SLACK = 5.f;  // log2: weights below 2^15 fit f16
 
 template <int N>
@@ -92,8 +96,10 @@ struct StepSmem {
   static_assert(ST_WARPS * R * D * 4 <= QF, "O staging fits the ring");
 };
 
+// (The CTAs per SM that the registers allow anyway, said to the compiler: 32 trees
+// of 8 tokens 42 us, 45 .. 47 without.)
 template <bool E4M3, int D, int NT, bool PS>
-__global__ void __launch_bounds__(ST_THREADS) kv8_step_kernel(const Kv8Args a, const int fused_append) {
+__global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1) kv8_step_kernel(const Kv8Args a, const int fused_append) {
   using L = StepShape<D>;
   using M = StepSmem<D, NT>;
   constexpr int R = M::R;
@@ -539,8 +545,10 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   // wave of CTAs that are resident together (three per SM for 8 query rows, two for
   // 16), at least 128 cache positions each, 16 CTAs at most; and two for calls of
   // between one and two waves of long rows, whose second wave would be mostly
-  // empty (64 sequences over 4096 .. 8191 positions: 179 us, 208 unsplit; 32 trees
-  // over 1500: 45 us unsplit, 61 and 66 with two and four).
+  // empty (measured before the last steps, 64 sequences over 4096 .. 8191 positions:
+  // 179 us, 208 unsplit; 32 trees over 1500: 45 us unsplit, 61 and 66 with two and
+  // four). Three sequences over 40000 (12 x 16 CTAs) are bound by the SMs that hold
+  // two CTAs: 40 us; clusters of 8, 9, 12 and 14: 50, 46, 50, 44.
   const int64_t ctas = (int64_t)a.B * a.KVH * tiles;
   const int64_t wave = (NT == 1 ? 3 : 2) * (int64_t)b2m::device_sm_count();
   int cl = 1;
