@@ -528,7 +528,7 @@ B2M_API b2m_status b2m_rotary_dev(b2m_ctx *ctx, const float *x, int64_t x_rs, co
  * reference, whose cache is float32 (lib/src/onnx_ops.dart:1844).
  *
  * One layer's cache: codes [b][kvh][cap][head_dim] (4-byte aligned), scales
- * [b][kvh][cap], device memory owned by the caller. head_dim <= 256. */
+ * [b][kvh][cap], device memory owned by the caller. head_dim <= 256, cap <= 2^30. */
 typedef struct b2m_kv8_cache {
   void *k, *v;
   float *k_scale, *v_scale;
@@ -541,7 +541,8 @@ typedef struct b2m_kv8_cache {
  * or the keys' head-norm gains [kvh][head_dim] (as the k rows of
  * b2m_gqa_qknorm_dev's qk_gain) with epsilon eps. depth: NULL (token i sits at
  * position past + i), or [b][s] int32: rotary position past + depth[i], for
- * drafted trees (0 <= depth[i] < s). cos / sin: [cap][rotary_half] or NULL.
+ * drafted trees (0 <= depth[i] < s; read for the rotary only). cos / sin:
+ * [cap][rotary_half] or NULL.
  * A token past the capacity is not written and raises the capacity error; a
  * negative past or a depth outside [0, s) is an index error and writes
  * nothing for that token (reported by the next synchronising call). */
@@ -565,10 +566,12 @@ B2M_API b2m_status b2m_kv8_read_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, co
  * and the new tokens j whose bit j is set (a token sees itself only if its
  * own bit is set; one that sees nothing gets zeros). out: [b][s] rows of
  * h*head_dim, and / or out16, the same rounded to f16 (h*head_dim % 8 == 0);
- * one of them may be NULL. Scale <= 0 means 1/sqrt(head_dim). fp32 rows carry
- * fp32 accuracy (operands split into two f16 terms on the tensor cores);
- * with out16 alone, q and the softmax weights are rounded to f16, below the
- * output's own rounding. EXACT attention mode (b2m_set_attention_mode) runs
+ * one of them may be NULL. Scale <= 0 means 1/sqrt(head_dim). With out, the
+ * queries and the softmax weights are split into two f16 terms on the tensor
+ * cores (about 1e-6 of the largest value of a row, 2.4e-6 over thousands of
+ * keys). With out16 alone one of the two is rounded to f16 once (the weights
+ * for calls of up to 48 query rows per kv head, the queries above): an error
+ * like that of the output's own rounding. EXACT attention mode (b2m_set_attention_mode) runs
  * the fp32 CUDA-core kernel. */
 B2M_API b2m_status b2m_gqa_kv8_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const float *q, const float *k,
                                    const float *v, int64_t q_rs, int64_t kv_rs, const float *qk_gain, double eps,

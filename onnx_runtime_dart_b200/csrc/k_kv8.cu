@@ -29,7 +29,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const Kv8Args a) {
 // The same for rows of whole float4s: half a warp per (token, kv head), both
 // sides. Bound by issue slots, not by memory (8 D bytes in, 2 D + 8 out): what a
 // row costs beside its elements (the norm factor, the maximum in double) is paid
-// once for two rows.
+// once for two rows. 16376 tokens of 8 kv heads of 128, normed and rotated, 73 us
+// (2.3 TB/s, issue slots 65% used; 103 us with a warp per row; floor 26).
 template <bool E4M3, int NCH>
 __global__ void __launch_bounds__(256, NCH == 4 ? 1 : 3) kv8_append_vec_kernel(const Kv8Args a) {
   pdl_launch_dependents();
@@ -41,7 +42,8 @@ __global__ void __launch_bounds__(256, NCH == 4 ? 1 : 3) kv8_append_vec_kernel(c
 }
 
 // The values of n cached positions from start[b] (or 0) on, [B][KVH][n][D]
-// fp32: one warp per row.
+// fp32: one warp per row. Bound by the stores (8 D bytes for 2 D + 8 read): 34 us
+// for 16376 tokens of 8 heads of 128, 5.0 TB/s; 52 us with one code a lane.
 template <bool E4M3>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Args a, const int32_t *start, int n, float *k_out,
                                                        float *v_out) {
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(256) kv8_attend_kernel(const Kv8Args a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int kvh = h / (a.H / a.KVH), D = a.D;
-  const int past = max(0, a.past[b]);
+  const int past = min(max(0, a.past[b]), a.CAP);  // (an append past either has raised its error)
   const int64_t pos = token_pos(a, b, i, past);
   float x = tid < D ? a.q[((int64_t)b * a.S + i) * a.q_rs + (int64_t)h * D + tid] : 0.f;
   if (a.q_gain) {

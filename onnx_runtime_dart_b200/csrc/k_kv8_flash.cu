@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   const int row0 = (int)(gridDim.z - 1 - blockIdx.z) * FL_ROWS;  // the longest rows of all first
   const int kvh = (int)(blockIdx.x / CL), b = blockIdx.y;
   const int G = a.H / a.KVH, nrows = a.S * G;
-  const int past = max(0, a.past[b]);
+  const int past = min(max(0, a.past[b]), a.CAP);  // (an append past either has raised its error)
   const int last_token = min(a.S - 1, (row0 + FL_ROWS - 1) / G);
   const int n = (int)min((int64_t)a.CAP, (int64_t)past + (a.tree ? a.S : last_token + 1));
   const int all_tiles = (n + FL_TILE - 1) / FL_TILE, per = (all_tiles + CL - 1) / CL;
@@ -380,7 +380,8 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         for (int part = QS ? 0 : 1; part < 2; part++)
 #pragma unroll
           for (int kk = 0; kk < D / 16; kk++) {
-            const uint64_t oq = ((kk >> 2) * 16384u + (kk & 3) * 32u) >> 4, ok = ((kk >> 2) * 8192u + (kk & 3) * 32u) >> 4;
+            const uint64_t oq = ((kk >> 2) * 16384u + (kk & 3) * 32u) >> 4,
+                           ok = ((kk >> 2) * 8192u + (kk & 3) * 32u) >> 4;
             umma_f16(ts, (part ? d_qh : d_ql) + oq, dk + ok, idesc_s, (QS && part) || kk ? 1u : 0u);
           }
         umma_commit(s_full + (t & 1));

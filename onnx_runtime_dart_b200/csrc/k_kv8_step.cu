@@ -99,7 +99,8 @@ struct StepSmem {
 // (The CTAs per SM that the registers allow anyway, said to the compiler: 32 trees
 // of 8 tokens 42 us, 45 .. 47 without.)
 template <bool E4M3, int D, int NT, bool PS>
-__global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1) kv8_step_kernel(const Kv8Args a, const int fused_append) {
+__global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
+    kv8_step_kernel(const Kv8Args a, const int fused_append) {
   using L = StepShape<D>;
   using M = StepSmem<D, NT>;
   constexpr int R = M::R;
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1) 
   const int g = lane >> 2, t = lane & 3;
   const int row0 = (int)(blockIdx.x / CL) * R, kvh = blockIdx.y, b = blockIdx.z;
   const int G = a.H / a.KVH, nrows = a.S * G;
-  const int past = max(0, a.past[b]);
+  const int past = min(max(0, a.past[b]), a.CAP);  // (an append past either has raised its error)
   // keys that the tile's last row sees
   const int n = (int)min((int64_t)a.CAP, (int64_t)past + (a.tree ? a.S : min(a.S, (row0 + R - 1) / G + 1)));
   const int chunk = (((n + CL - 1) / CL) + 15) & ~15;

@@ -13,13 +13,15 @@
 // logit's order-preserving bits over the complement of its index, so equal
 // logits fall to the lowest index. An entry is looked at only when it reaches
 // a threshold that k entries of the CTA are known to reach, first from the
-// threads' maxima of the first batch, then from the warps' lists. Such entries go to a buffer of the warp that is sorted and merged
-// into its list when 32 are in it. No barrier stands in the loop.
+// threads' maxima of the first batch, then from the warps' lists. Such entries go
+// to a buffer of the warp that is sorted and merged into its list when 32 are in
+// it. No barrier stands in the loop.
 //
 // Bound by HBM: 4 V bytes per row are read once, about eight issue slots and
 // one MUFU operation per entry. Measured on one B200, 1024 rows of 151936: 97 us
-// without alternatives (6.4 TB/s), 116 us with k = 1, 131 us with k = 20; one
-// row 5.6 and 12.2 us.
+// without alternatives (6.4 TB/s), 116 us with k = 1, 131 us with k = 20 (issue
+// slots 73% used); one row over a cluster of 16 CTAs 10.5 us with k = 20 (launch, cluster and the
+// merge of the lists; its bytes would take 0.1 us).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -39,7 +41,7 @@ constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_VEC = 4;     // float4 loads of a thread per batch
 constexpr int LP_FLUSH = 32;  // buffered keys of a warp that are worth a merge
 constexpr int LP_BUF = LP_FLUSH - 1 + 32 * 4 * LP_VEC;  // what a flush leaves and one batch
-constexpr int LP_CTAS = 4;     // resident per SM
+constexpr int LP_CTAS = 4;    // resident per SM
 constexpr int LP_MAX_CLUSTER = 16;  // above 8: opted in for the kernel
 typedef unsigned long long u64;
 

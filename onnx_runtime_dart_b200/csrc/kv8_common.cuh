@@ -118,9 +118,9 @@ __device__ __forceinline__ void quantise_row(const float *xs, int D, const float
 // Rotary position of new token i of sequence b; -1 when its depth is outside
 // [0, S) (the caller raises the device error).
 __device__ __forceinline__ int64_t token_pos(const Kv8Args &a, int b, int i, int past) {
-  if (!a.depth) return past + i;
+  if (!a.depth) return (int64_t)past + i;
   const int dp = a.depth[(int64_t)b * a.S + i];
-  return dp < 0 || dp >= a.S ? -1 : past + dp;
+  return dp < 0 || dp >= a.S ? -1 : (int64_t)past + dp;
 }
 
 // Quantises one side (0: key, 1: value) of new token i of (sequence b, kv head)

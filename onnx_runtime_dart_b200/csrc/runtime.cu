@@ -2092,7 +2092,7 @@ static Kv8Args kv8_cache_args(const b2m_kv8_cache *c, bool used, const char *wha
   B2M_REQUIRE(c, B2M_ERR_INVALID_ARGUMENT, w + ": cache is null");
   B2M_REQUIRE(c->type == B2M_INT8 || c->type == B2M_FLOAT8E4M3FN, B2M_ERR_UNSUPPORTED,
               w + ": the cache type must be INT8 or FLOAT8E4M3FN");
-  B2M_REQUIRE(c->b >= 0 && c->kvh > 0 && c->cap > 0 && c->head_dim > 0 && c->head_dim <= 256,
+  B2M_REQUIRE(c->b >= 0 && c->kvh > 0 && c->cap > 0 && c->cap <= (1 << 30) && c->head_dim > 0 && c->head_dim <= 256,
               B2M_ERR_INVALID_ARGUMENT, w + ": bad cache shape");
   B2M_REQUIRE(!used || (c->k && c->v && c->k_scale && c->v_scale), B2M_ERR_INVALID_ARGUMENT,
               w + ": null cache pointer");

@@ -495,6 +495,25 @@ def test_attend_capacity(ctx):
     ctx.synchronize()
 
 
+@pytest.mark.parametrize("s,d,tree", [(1, 128, False), (6, 64, False), (40, 128, False), (40, 64, True), (3, 36, False)])
+def test_positions_at_the_ends_of_int32(ctx, s, d, tree):
+    """Positions far outside the cache: the error, no row written, the other sequence's rows right."""
+    p = Problem("e4m3", 3, s, 4, 2, d, 128, [20, 20, 20], rot=32, half=16)
+    if tree:
+        p.depth = torch.arange(s, dtype=torch.int32, device="cuda").repeat(3, 1)
+        p.tree = torch.full((3, s), 1, dtype=torch.int64, device="cuda")
+    for bad, what in ((2**31 - 1, "capacity"), (-(2**31), "index")):
+        p.past[:] = torch.tensor([20, bad, 20], dtype=torch.int32)
+        was = [t[1].clone() for t in p.codes + p.scales]
+        p.attend(ctx)
+        with pytest.raises(N.ArgumentError, match=what):
+            ctx.synchronize()
+        assert all(torch.equal(t[1].view(torch.uint8), w.view(torch.uint8)) for t, w in zip(p.codes + p.scales, was))
+        p.past[1] = 20
+        want, tol, _ = p.answer()
+        assert bool(((p.out.double() - want).abs() <= tol)[[0, 2]].all())
+
+
 @pytest.mark.parametrize("b,s,h,kvh,d", [(3, 1, 16, 8, 128), (2, 12, 8, 2, 64), (1, 150, 4, 2, 128)])
 def test_graph_replay_and_other_stream(ctx, b, s, h, kvh, d):
     """Captured on a side stream and replayed with new inputs and positions: the same bits as eager calls."""

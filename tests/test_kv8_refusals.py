@@ -44,6 +44,7 @@ BAD_CACHES = [(dict(type=N.B2M_FLOAT), N.UnsupportedError, "cache type"),
               (dict(type=N.B2M_UINT8), N.UnsupportedError, "cache type"),
               (dict(head_dim=257), N.ArgumentError, "cache shape"), (dict(head_dim=0), N.ArgumentError, "cache shape"),
               (dict(cap=0), N.ArgumentError, "cache shape"), (dict(kvh=0), N.ArgumentError, "cache shape"),
+              (dict(cap=(1 << 30) + 1), N.ArgumentError, "cache shape"),
               (dict(b=-1), N.ArgumentError, "cache shape"), (dict(k=0), N.ArgumentError, "null cache"),
               (dict(v_scale=0), N.ArgumentError, "null cache"), (dict(k=P + 2), N.ArgumentError, "4-byte"),
               (dict(v=P + 1), N.ArgumentError, "4-byte")]
