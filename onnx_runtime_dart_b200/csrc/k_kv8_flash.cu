@@ -332,18 +332,34 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
       mbar_arrive(k_full + kst);
       return true;
     };
+    // The append of the call's rows may still run: tiles without new rows go ahead
+    // (what came before the append is visible: it was launched without an early start).
+    bool appended = false;
+    auto reach = [&](int t) {
+      if (!appended && (t0 + t + 1) * (int64_t)FL_TILE > past) {
+        pdl_wait();
+        appended = true;
+      }
+    };
     if (ntile > 0) {
+      reach(0);
       load_k(0);
       load_v(0);
       put_k(0);
-      if (ntile > 1) load_k(1);
+      if (ntile > 1) {
+        reach(1);
+        load_k(1);
+      }
     }
     // K_{t+1} before V_t: its products are wanted first (under tile t's softmax).
 #pragma unroll 1
     for (int t = 0; t < ntile; t++) {
       if (t + 1 < ntile) {
         if (!put_k(t + 1)) break;
-        if (t + 2 < ntile) load_k(t + 2);
+        if (t + 2 < ntile) {
+          reach(t + 2);
+          load_k(t + 2);
+        }
       }
       const int vst = t % L::VST;
       if (t >= L::VST && !warp_wait_phase(v_empty + vst, (uint32_t)(t / L::VST - 1) & 1u, abort_flag, a.err)) break;
@@ -605,6 +621,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   else
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FL_REGS));
   if (CL > 1) cluster.sync();
+  pdl_wait();  // no CTA ends before the append it was launched beside
   // Rows to memory, a cluster's ranks sharing them.
   const float *o_s = reinterpret_cast<const float *>(smem);
   constexpr int D4 = D / 4;
@@ -696,12 +713,14 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   cfg.blockDim = dim3(FL_THREADS);
   cfg.dynamicSmemBytes = L::BYTES;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)cl;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // starts beside the call's append
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   B2M_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
 }
 
@@ -724,7 +743,7 @@ bool kv8_flash_shape(const Kv8Args &a) {
          al(a.kc, 16) && al(a.vc, 16) && al(a.out, 16) && al(a.out16, 8);
 }
 
-// The call's keys and values must have been appended.
+// The launch before this one must be that of the call's append.
 void launch_kv8_flash(const Kv8Args &a, cudaStream_t s) {
   if (a.e4m3) {
     if (a.D == 128)

@@ -170,11 +170,12 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
   };
 
   // The first tiles are on their way while the rows below are prepared (a tile
-  // with rows that this call still appends waits for them).
+  // with rows that this call still appends waits for them). Of what came before
+  // the append all is visible: the append was launched without an early start.
   int ahead = 0;
 #pragma unroll
   for (int k = 0; k < ST_STAGES - 1; k++)
-    if (ahead == k && (!fused_append || jbeg + 16 * (warp + k * ST_WARPS) + 16 <= past)) {
+    if (ahead == k && jbeg + 16 * (warp + k * ST_WARPS) + 16 <= past) {
       issue(warp + k * ST_WARPS, k);
       ahead = k + 1;
     }
@@ -215,6 +216,7 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
       }
     }
     __syncthreads();
+    b2m::pdl_wait();  // an append launched before this kernel is through
 #pragma unroll
     for (int k = 0; k < ST_STAGES - 1; k++)
       if (k >= ahead) issue(warp + k * ST_WARPS, k);
@@ -561,12 +563,14 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   cfg.blockDim = dim3(ST_THREADS);
   cfg.dynamicSmemBytes = M::BYTES;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)cl;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // starts beside its own append
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = fused ? 1 : 2;
   B2M_CUDA(cudaLaunchKernelEx(&cfg, kern, a, fused ? 1 : 0));
 }
 
