@@ -212,37 +212,42 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   }
   if (warp == 8) tmem_alloc(slot, 256);
 
-#pragma unroll 1
-  for (int rr = warp * 4 + (lane >> 3); rr < FL_ROWS; rr += FL_THREADS / 8) {
-    QRow<D> q;
-    load_q_row<D>(a, b, kvh, G, row0 + rr, past, q);
-#pragma unroll
-    for (int u = 0; u < D / 32; u++) {
-      const int d = 4 * ((lane & 7) + 8 * u);
-      // (in the order of K's expanded codes)
-      const float v[4] = {q.v[u].x, q.v[u].y, q.v[u].z, q.v[u].w};
-      const float4 x = make_float4(v[0], v[expand_order<E4M3>(1)], v[expand_order<E4M3>(2)], v[3]);
-      const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
-      const uint32_t at = (uint32_t)(d >> 6) * 16384u + sw128(rr, d & 63);
-      *reinterpret_cast<uint2 *>(smem + L::QH + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
-      if (QS) {
-        const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
-        *reinterpret_cast<uint2 *>(smem + L::QL + at) =
-            make_uint2(h2_as_u32(__floats2half2_rn(x.x - g0.x, x.y - g0.y)),
-                       h2_as_u32(__floats2half2_rn(x.z - g1.x, x.w - g1.y)));
-      }
-    }
-    if ((lane & 7) == 0) {
-      row_factor[rr] = q.factor;
-      row_lim[rr] = q.lim;
-      row_bits[rr] = q.bits;
-    }
-  }
-  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *slot, 0);
+
+  // The query rows, by the warps that will use them; the others start on the tiles.
+  if (warp < 4 || warp >= 8) {
+#pragma unroll 1
+    for (int rr = (warp < 4 ? warp : warp - 4) * 4 + (lane >> 3); rr < FL_ROWS; rr += 32) {
+      QRow<D> q;
+      load_q_row<D>(a, b, kvh, G, row0 + rr, past, q);
+#pragma unroll
+      for (int u = 0; u < D / 32; u++) {
+        const int d = 4 * ((lane & 7) + 8 * u);
+        // (in the order of K's expanded codes)
+        const float v[4] = {q.v[u].x, q.v[u].y, q.v[u].z, q.v[u].w};
+        const float4 x = make_float4(v[0], v[expand_order<E4M3>(1)], v[expand_order<E4M3>(2)], v[3]);
+        const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
+        const uint32_t at = (uint32_t)(d >> 6) * 16384u + sw128(rr, d & 63);
+        *reinterpret_cast<uint2 *>(smem + L::QH + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
+        if (QS) {
+          const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
+          *reinterpret_cast<uint2 *>(smem + L::QL + at) =
+              make_uint2(h2_as_u32(__floats2half2_rn(x.x - g0.x, x.y - g0.y)),
+                         h2_as_u32(__floats2half2_rn(x.z - g1.x, x.w - g1.y)));
+        }
+      }
+      if ((lane & 7) == 0) {
+        row_factor[rr] = q.factor;
+        row_lim[rr] = q.lim;
+        row_bits[rr] = q.bits;
+      }
+    }
+    fence_proxy_async_smem();
+    named_barrier_sync(1, FL_THREADS - 128);
+  }
 
   if (warp >= 4 && warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FL_REGS_TILES));
@@ -625,15 +630,26 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   // Rows to memory, a cluster's ranks sharing them.
   const float *o_s = reinterpret_cast<const float *>(smem);
   constexpr int D4 = D / 4;
+  const int rows = *abort_flag ? 0 : min(FL_ROWS, nrows - row0);  // (a wait that gave up: nothing)
+  auto put = [&](int rr, int c, const float4 &acc) {
+    const int r = row0 + rr;
+    const int64_t at = ((int64_t)b * a.S + r / G) * a.H * D + (int64_t)(kvh * G + r % G) * D + 4 * c;
+    if (a.out) *reinterpret_cast<float4 *>(a.out + at) = acc;
+    if (a.out16) {
+      const __half2 h0 = __floats2half2_rn(acc.x, acc.y), h1 = __floats2half2_rn(acc.z, acc.w);
+      *reinterpret_cast<uint2 *>(a.out16 + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
+    }
+  };
+  if (CL == 1) {
+#pragma unroll 4
+    for (int e = tid; e < rows * D4; e += FL_THREADS)
+      put(e / D4, e % D4, *reinterpret_cast<const float4 *>(o_s + e / D4 * L::OST + 4 * (e % D4)));
+  } else {
 #pragma unroll 1
-  for (int e = rank * FL_THREADS + tid; e < FL_ROWS * D4; e += CL * FL_THREADS) {
-    const int rr = e / D4, c = e % D4, r = row0 + rr;
-    if (r >= nrows || *abort_flag) continue;
-    const float *src = o_s + rr * L::OST + 4 * c;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (CL == 1) {
-      acc = *reinterpret_cast<const float4 *>(src);
-    } else {
+    for (int e = rank * FL_THREADS + tid; e < rows * D4; e += CL * FL_THREADS) {
+      const int rr = e / D4, c = e % D4;
+      const float *src = o_s + rr * L::OST + 4 * c;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       // four ranks at once, their loads ahead of the first use (one after the other: 56 us for 53)
       float top = -INFINITY, sum = 0.f;
       for (int q0 = 0; q0 < CL; q0 += 4) {
@@ -664,12 +680,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-    }
-    const int64_t at = ((int64_t)b * a.S + r / G) * a.H * D + (int64_t)(kvh * G + r % G) * D + 4 * c;
-    if (a.out) *reinterpret_cast<float4 *>(a.out + at) = acc;
-    if (a.out16) {
-      const __half2 h0 = __floats2half2_rn(acc.x, acc.y), h1 = __floats2half2_rn(acc.z, acc.w);
-      *reinterpret_cast<uint2 *>(a.out16 + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
+      put(rr, c, acc);
     }
   }
   if (CL > 1) cluster.sync();  // the others have read this CTA's rows
