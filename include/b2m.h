@@ -570,7 +570,7 @@ B2M_API b2m_status b2m_kv8_read_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, co
  * queries and the softmax weights are split into two f16 terms on the tensor
  * cores (about 1e-6 of the largest value of a row, 2.4e-6 over thousands of
  * keys). With out16 alone one of the two is rounded to f16 once (the weights
- * for calls of up to 48 query rows per kv head, the queries above): an error
+ * for calls of few query rows per kv head, the queries for many): an error
  * like that of the output's own rounding. EXACT attention mode (b2m_set_attention_mode) runs
  * the fp32 CUDA-core kernel. */
 B2M_API b2m_status b2m_gqa_kv8_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const float *q, const float *k,

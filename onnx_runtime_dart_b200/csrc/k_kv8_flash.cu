@@ -745,12 +745,16 @@ void launch_out(const Kv8Args &a, cudaStream_t s) {
 
 }  // namespace
 
-// Enough rows to fill most of a 128-row tile, head dims and alignments the
-// kernel takes.
+// Enough rows, head dims and alignments the kernel takes. The other kernel reads
+// the cache once per 16 rows: above 48 rows this one is faster however few CTAs
+// there are, from 33 on where the other's CTAs are more than one wave (32 x 8
+// (sequence, kv head)s over 1500 keys: 40 rows 74 us, 99 there, 48 rows 75 and 100;
+// 32 rows 72 and 69. With 2 x 8 over 6000 keys 48 rows take 45 and 37).
 bool kv8_flash_shape(const Kv8Args &a) {
   auto al = [](const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   const int64_t rows = (int64_t)a.S * (a.H / a.KVH);
-  return (a.D == 64 || a.D == 128) && rows > 48 && rows <= 65535 * FL_ROWS && a.KVH <= 65535 && q_rows_vec(a) &&
+  const bool enough = rows > 48 || (rows > 32 && (int64_t)a.B * a.KVH * 3 > 2 * (int64_t)device_sm_count());
+  return (a.D == 64 || a.D == 128) && enough && rows <= 65535 * FL_ROWS && a.KVH <= 65535 && q_rows_vec(a) &&
          al(a.kc, 16) && al(a.vc, 16) && al(a.out, 16) && al(a.out16, 8);
 }
 

@@ -358,6 +358,7 @@ CHUNKS = [  # b, s, h, kvh, d, cap, past, rot, inter, norm
     (1, 21, 4, 2, 80, 50, 9, 80, False, True),
     (1, 200, 12, 1, 128, 260, 50, 128, False, False),
     (1, 9, 3, 1, 32, 20, 2, 0, False, False),
+    (25, 20, 8, 4, 64, 80, 50, 64, False, True),     # 40 rows of many kv heads
 ]
 
 
@@ -393,6 +394,7 @@ TREES = [  # b, n, h, kvh, d, cap, past, rot, norm, orphan
     (1, 40, 8, 1, 256, 100, 31, 0, False, True),
     (2, 5, 3, 1, 32, 12, 7, 32, False, False),
     (2, 12, 12, 4, 96, 90, 64, 96, True, True),
+    (13, 24, 16, 8, 128, 100, 70, 128, True, True),  # 48 rows of many kv heads
 ]
 
 
