@@ -497,6 +497,33 @@ def test_attend_capacity(ctx):
     ctx.synchronize()
 
 
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+@pytest.mark.parametrize("s,d", [(1, 128), (5, 64), (40, 128)])
+def test_keys_at_odd_strides(ctx, kv, s, d):
+    """Keys and values in buffers of their own, unaligned and with an odd row stride: the packed rows' answers."""
+    p = Problem(kv, 2, s, 8, 2, d, 160, [70, 33], d, False, True)
+    nk = p.kvh * d
+    bufs = []
+    for side in range(2):
+        o = (p.h + side * p.kvh) * d
+        t = torch.full((2 * s * (nk + 3) + 1,), float("nan"), device="cuda")
+        t[1:].view(2 * s, nk + 3)[:, :nk] = p.rows[:, o: o + nk]
+        bufs.append(t)
+    p.out = torch.full((2, s, 8 * d), 7.0, device="cuda")
+    N.check(ctx.lib.b2m_gqa_kv8_dev(ctx.handle, ctypes.byref(p.cache), _p(p.rows), _p(bufs[0], 4), _p(bufs[1], 4), p.rs,
+                                    nk + 3, _p(p.gain), 1e-6, _p(p.past), None, None, *p.rotary(), _p(p.out), None, s,
+                                    p.h, ctypes.c_float(0.0)))
+    ctx.synchronize()
+    want, tol, _ = p.answer()
+    assert bool(((p.out.double() - want).abs() <= tol).all())
+    new = p.new_rows()
+    for side in range(2):
+        for i in range(2):
+            at = int(p.past[i])
+            assert torch.equal(_decode(p.codes[side][i, :, at: at + s], kv), new[side][0][i])
+            assert torch.equal(p.scales[side][i, :, at: at + s], new[side][1][i].float())
+
+
 @pytest.mark.parametrize("s,d,tree", [(1, 128, False), (6, 64, False), (40, 128, False), (40, 64, True), (3, 36, False)])
 def test_positions_at_the_ends_of_int32(ctx, s, d, tree):
     """Positions far outside the cache: the error, no row written, the other sequence's rows right."""
