@@ -1305,7 +1305,6 @@ __device__ __forceinline__ void mtc_stage_rows(uint8_t *smem, uint32_t off_h, ui
 // column block w / 4: 32 of the 128 score columns, 16 of the 64 output
 // columns; row max and sum combine the four column blocks in shared memory.
 __global__ void __launch_bounds__(512) mha_tc_kernel(const GqaArgs a) {
-  b2m::pdl_launch_dependents();
   extern __shared__ uint8_t mtc_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(mtc_raw) + 1023) & ~(uintptr_t)1023);
   float *mrow = reinterpret_cast<float *>(smem + MTC_MASK);
@@ -1365,6 +1364,7 @@ __global__ void __launch_bounds__(512) mha_tc_kernel(const GqaArgs a) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *slot;
+  b2m::pdl_launch_dependents();  // behind the allocation: a dependent must not take TMEM first and wait for this grid
   if (tid == 0) {
     constexpr uint32_t idesc_s = umma_idesc(128, 128, 1u, 1u, 1u);
     const uint32_t base = smem_u32(smem);
@@ -1527,7 +1527,6 @@ struct FaLayout {
 
 template <int D>
 __global__ void __launch_bounds__(512, 1) fa_tc_kernel(const GqaArgs a) {
-  b2m::pdl_launch_dependents();
   using L = FaLayout<D>;
   constexpr int DW = D / 4;  // output columns per thread
   extern __shared__ uint8_t fa_raw[];
@@ -1684,6 +1683,7 @@ __global__ void __launch_bounds__(512, 1) fa_tc_kernel(const GqaArgs a) {
     *reinterpret_cast<uint4 *>(smem + L::QL + o) = lv;
   }
   __syncthreads();  // the Q staging scratch is consumed before K / V reuse it
+  b2m::pdl_launch_dependents();  // behind the TMEM allocation, as in mha_tc_kernel
 
   const int nkeys = min(past + a.S, a.CAP);
   const int kend = min(nkeys, past + min(q0 + 128, a.S));  // keys any row of the tile sees

@@ -184,7 +184,6 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::SLOT);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::FLAG);
 
-  pdl_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tid = threadIdx.x;
@@ -218,6 +217,10 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *slot, 0);
+  // Behind the allocation: a dependent kernel that fits beside this CTA and wants
+  // all of TMEM could otherwise take it first and then wait for this grid, which
+  // would wait for TMEM.
+  pdl_launch_dependents();
 
   // The query rows, by the warps that will use them; the others start on the tiles.
   if (warp < 4 || warp >= 8) {
