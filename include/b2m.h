@@ -566,7 +566,9 @@ B2M_API b2m_status b2m_kv8_read_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, co
  * and the new tokens j whose bit j is set (a token sees itself only if its
  * own bit is set; one that sees nothing gets zeros). out: [b][s] rows of
  * h*head_dim, and / or out16, the same rounded to f16 (h*head_dim % 8 == 0);
- * one of them may be NULL. Scale <= 0 means 1/sqrt(head_dim). With out, the
+ * one of them may be NULL. Scale <= 0 means 1/sqrt(head_dim). A token's result
+ * keeps its digits whatever the value rows that it does not see, or hardly
+ * weighs, hold, as long as they are below 2^85 times those that it does. With out, the
  * queries and the softmax weights are split into two f16 terms on the tensor
  * cores (about 1e-6 of the largest value of a row, 2.4e-6 over thousands of
  * keys). With out16 alone one of the two is rounded to f16 once (the weights

@@ -13,8 +13,11 @@
 //              work under the softmax;
 //   warps 0-3  a thread per query row (= TMEM lane): scores times K's scale,
 //              the causal or tree mask, exp2 against a reference that only moves
-//              when a score passes it by 2^5 (O in TMEM is rescaled then), the
-//              weights times V's scale as f16 back into S's columns.
+//              when a weight would pass 2^15 (O in TMEM is rescaled then), the
+//              weights times V's scale as f16 back into S's columns. V's scales
+//              are kept over the largest of the CTA's keys, hidden ones included;
+//              the reference goes by what the row itself sees (weight_ref), which
+//              costs extra operations only in tiles with a scale below 2^-8 of that.
 // No cross-thread reduction is left in the softmax. Two CTAs share an SM, so one's
 // exponentials run under the other's products.
 //
@@ -24,7 +27,7 @@
 // both split, 3.5e-4 with neither; 259, 281 and 250 us for 4 x 2048 tokens).
 //
 // Few row tiles over many keys (a tree on long sequences): the CTAs of a cluster
-// split the keys and merge their O, m and l through distributed shared memory in
+// split the keys and merge their O, reference and l through distributed shared memory in
 // rank order; no workspace, no atomics.
 //
 // 4 x 2048 causal tokens (16 heads on 8) take 235 us with their append: 292 TFLOP/s
@@ -55,7 +58,6 @@ constexpr int FL_MAX_CLUSTER = 8, FL_THREADS = 384, FL_TILE = 64, FL_ROWS = 128,
 // what it was launched with: the roles' sum is no more.
 constexpr int FL_REGS = 80, FL_REGS_SOFTMAX = 136, FL_REGS_TILES = 64, FL_REGS_MMA = 40;
 static_assert(FL_REGS_SOFTMAX + FL_REGS_TILES + FL_REGS_MMA <= 3 * FL_REGS, "register split");
-constexpr float FL_BIAS = 10.f, FL_SLACK = 5.f;  // log2: weights stay below 2^15
 
 __device__ __forceinline__ uint32_t sw128(int r, int k) {  // byte offset of 16-bit element k < 64 of row r
   return (uint32_t)(r * 128 + ((((k >> 3) ^ (r & 7)) << 4) | ((k & 7) << 1)));
@@ -155,10 +157,10 @@ struct FlashLayout {
   // O staging [128][D + 4] fp32 at the end, over Q, K and V
   static constexpr int OST = D + 4;
   static constexpr uint32_t SCALES0 = 128 * OST * 4 > TILES ? 128 * OST * 4 : TILES;
-  // ks[SLOTS][64], vs[SLOTS][64], vf[SLOTS], vnan[SLOTS], vref; then per row: factor, limit,
-  // bits, m, l; barriers
+  // ks[SLOTS][64], vs[SLOTS][64], vf[SLOTS], vflag[SLOTS], vref; then per row: factor, limit,
+  // bits, reference, l; barriers
   static constexpr uint32_t SCALES = SCALES0;
-  static constexpr uint32_t VF = SCALES + FL_SLOTS * 64 * 8, VNAN = VF + FL_SLOTS * 4, VREF = VNAN + FL_SLOTS * 4;
+  static constexpr uint32_t VF = SCALES + FL_SLOTS * 64 * 8, VFLAG = VF + FL_SLOTS * 4, VREF = VFLAG + FL_SLOTS * 4;
   static constexpr uint32_t ROWS = VREF + 16;
   static constexpr uint32_t BARS = ROWS + 128 * (8 + 4 + 4 + 4 + 4);
   static constexpr uint32_t SLOT = BARS + 14 * 8, FLAG = SLOT + 4;
@@ -173,11 +175,11 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   extern __shared__ __align__(1024) uint8_t smem[];
   float *ks_s = reinterpret_cast<float *>(smem + L::SCALES), *vs_s = ks_s + FL_SLOTS * 64;
   float *vf_s = reinterpret_cast<float *>(smem + L::VF), *vref_s = reinterpret_cast<float *>(smem + L::VREF);
-  int *vnan_s = reinterpret_cast<int *>(smem + L::VNAN);
+  int *vflag_s = reinterpret_cast<int *>(smem + L::VFLAG);  // bit 0: a NaN scale, bit 1: one far below vref
   uint64_t *row_bits = reinterpret_cast<uint64_t *>(smem + L::ROWS);
   float *row_factor = reinterpret_cast<float *>(row_bits + 128);
   int *row_lim = reinterpret_cast<int *>(row_factor + 128);
-  float *row_m = reinterpret_cast<float *>(row_lim + 128), *row_l = row_m + 128;
+  float *row_ref = reinterpret_cast<float *>(row_lim + 128), *row_l = row_ref + 128;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BARS);
   uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8,
            *p_full = bars + 10, *o_done = bars + 12, *all_done = bars + 13;
@@ -332,8 +334,9 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         else
           vs_s[sl * 64 + 32 + lane] = sc[1] * vinv;
         const bool nan = __any_sync(0xffffffffu, sc[0] != sc[0] || sc[1] != sc[1]);
+        const bool low = __any_sync(0xffffffffu, !(sc[0] * vinv >= V_LOW) || !(sc[1] * vinv >= V_LOW));
         if (cw == 2 && lane == 0) {
-          vnan_s[sl] = nan;
+          vflag_s[sl] = (nan ? 1 : 0) | (low ? 2 : 0);
           vf_s[sl] = vf;
           *vref_s = vref;
         }
@@ -459,7 +462,9 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     const int lim = row_lim[rr];
     const uint64_t bits = row_bits[rr];
     const int all_see = a.tree ? past : past + row0 / G + 1;  // keys below this are seen by every row
-    float m = -INFINITY, mref = 0.f, l = 0.f;
+    // Largest score seen, log2 of the largest weight times V scale (at the reference
+    // weight 1), the reference the weights are taken against, their sum.
+    float m = -INFINITY, c_max = -INFINITY, ref = 0.f, l = 0.f;
     bool ok = true;
 #pragma unroll 1
     for (int t = 0; t < ntile; t++) {
@@ -516,15 +521,33 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         xm = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3])) * rf;  // rf > 0; -inf stays
       }
       const float vf = vf_s[sl];
-      if (__any_sync(0xffffffffu, xm > m + FL_SLACK || vf != 1.f)) {
-        const float mn = fmaxf(m, xm);
+      const int vflag = vflag_s[sl];
+      const ulonglong2 *vp = reinterpret_cast<const ulonglong2 *>(vs_s + sl * 64);
+      float cm = xm;  // the row's largest score + log2(V scale); exact where the tile's scales differ much
+      if (vflag & 2) {
+        cm = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < FL_TILE / 4; c++) {
+          const ulonglong2 v4 = vp[c];
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            float x0, x1, v0, v1;
+            unpack2(x[2 * c + k], x0, x1);
+            unpack2(k ? v4.y : v4.x, v0, v1);
+            cm = max3(cm, fmaf(x0, rf, lg2(v0)), fmaf(x1, rf, lg2(v1)));  // (a hidden key's NaN is passed over)
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, cm > c_max + REF_SLACK || xm > m + REF_SLACK || vf != 1.f)) {
         float f = vf;
-        if (mn > m) {
-          const float fm = m == -INFINITY ? 0.f : ex2(m - mn);
-          l = l == 0.f ? 0.f : l * fm;
-          f *= fm;
+        const float mn = fmaxf(m, xm);
+        if (mn > -INFINITY) {
+          c_max = fmaxf(c_max + lg2(vf), cm);
+          const float rn = weight_ref(mn, c_max), fr = m == -INFINITY ? 0.f : ex2(ref - rn);
+          l = l == 0.f ? 0.f : l * fr;
+          f *= fr;
           m = mn;
-          mref = mn - FL_BIAS;
+          ref = rn;
         }
         if (t > 0) {  // O holds the tiles before: rescale it once their products are done
           ok = warp_wait_phase(o_done, (uint32_t)(t - 1) & 1u, abort_flag, a.err);
@@ -548,8 +571,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           tmem_st_wait();
         }
       }
-      const ulonglong2 *vp = reinterpret_cast<const ulonglong2 *>(vs_s + sl * 64);
-      const f32x2 rf2 = pack2(rf, rf), mr2 = pack2(-mref, -mref);
+      const f32x2 rf2 = pack2(rf, rf), mr2 = pack2(-ref, -ref);
       uint32_t ph[32], pl[PS ? 32 : 1];
       f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
@@ -571,7 +593,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           }
         }
       }
-      if (vnan_s[sl] && !whole) {
+      if ((vflag & 1) && !whole) {
         // A key that this row does not see has a NaN scale: its weight is nothing.
         const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
 #pragma unroll
@@ -596,7 +618,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     }
     if (ok && ntile > 0) ok = warp_wait_phase(all_done, 0u, abort_flag, a.err);
     tc_fence_after();
-    // O (in the values' own scale), m and l to shared memory: Q, K and V are no
+    // O (in the values' own scale), reference and l to shared memory: Q, K and V are no
     // longer read (the last products have completed).
     float *ost = reinterpret_cast<float *>(smem) + rr * L::OST;
     if (ok) {
@@ -617,7 +639,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
                         : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
-    row_m[rr] = m;
+    row_ref[rr] = m == -INFINITY ? -INFINITY : ref;
     row_l[rr] = l;
   }
   // All roles meet before any takes registers back: a warp that gave its up and
@@ -666,14 +688,14 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           const int q = q0 + k;
           sm[k] = -INFINITY, sl[k] = 0.f, v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (q < CL) {
-            sm[k] = *cluster.map_shared_rank(row_m + rr, q);
+            sm[k] = *cluster.map_shared_rank(row_ref + rr, q);
             sl[k] = *cluster.map_shared_rank(row_l + rr, q);
             v[k] = *cluster.map_shared_rank(reinterpret_cast<const float4 *>(src), q);
           }
         }
 #pragma unroll
         for (int k = 0; k < 4; k++) top = fmaxf(top, sm[k]);
-        // none if a rank saw no key; with a NaN sum and no maximum the NaN is passed on
+        // none if a rank saw no key; with a NaN sum and no reference the NaN is passed on
         const float keep = sum == 0.f ? 0.f : (was == -INFINITY ? 1.f : ex2(was - top));
         sum *= keep, acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
 #pragma unroll

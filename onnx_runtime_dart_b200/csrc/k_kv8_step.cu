@@ -25,9 +25,10 @@
 // tile ahead 184 us, three 169; four CTAs per SM instead of three 184, six warps
 // per CTA 185, eight 223).
 //
-// The softmax reference m moves only when a score passes it by more than 2^5 (a
-// warp vote); weights are scaled by 2^10 so that f16 keeps small ones. V scales
-// are taken relative to the largest seen (2^ev). Warps, then the cluster's CTAs,
+// V scales are taken relative to the largest the warp has met (a power of two). A
+// row's softmax reference goes by its own largest weight times V scale (weight_ref)
+// and moves only when one passes 2^15, or in tiles with a V scale below 2^-8 (a warp
+// vote). Warps, then the cluster's CTAs,
 // merge in a fixed order through (distributed) shared memory: no workspace and
 // no atomics, so captured graphs share nothing and results repeat.
 #include <cooperative_groups.h>
@@ -43,7 +44,6 @@ namespace cg = cooperative_groups;
 using namespace kv8;
 
 constexpr int ST_WARPS = 4, ST_THREADS = 32 * ST_WARPS, ST_STAGES = 3;
-constexpr float P_BIAS = 10.f, M_SLACK = 5.f;  // log2: weights below 2^15 fit f16
 
 template <int N>
 __device__ __forceinline__ void cp_async(void *dst, const void *src) {
@@ -90,7 +90,7 @@ struct StepSmem {
   static constexpr int RING = 0;
   static constexpr int QF = RING + ST_WARPS * ST_STAGES * StepShape<D>::SLOT;  // Q fragments [NT][KSTEPS][32] uint4
   static constexpr int ROWS = QF + NT * StepShape<D>::KSTEPS * 512;            // per-row words, below
-  // bits[R] (u64), factor[R], lim[R], wm[4][R], wl[4][R], cm[R], cl[R]
+  // bits[R] (u64), factor[R], lim[R], wm[4][R], wl[4][R], cm[R], cl[R] (m: references)
   static constexpr int BYTES = ROWS + R * (8 + 4 + 4 + 16 + 16 + 8);
   // Warp states O [4][R][D] fp32 reuse the ring (drained by then).
   static_assert(ST_WARPS * R * D * 4 <= QF, "O staging fits the ring");
@@ -226,7 +226,9 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
   // cores cut off what an addition to a sum leaves below it, always toward zero,
   // and half as many additions to the large sums halve that.
   float o[NT][L::MT][4], ol[PS ? NT : 1][PS ? L::MT : 1][4];
-  float m[NT][2], mref[NT][2], l[NT][2], rf[NT][2];
+  // Per row: the largest score seen, log2 of the largest weight times V scale (at
+  // reference weight 1), the reference, the weights' sum, the scores' factor.
+  float m[NT][2], c_max[NT][2], ref[NT][2], l[NT][2], rf[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -238,8 +240,8 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
       }
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      m[nt][u] = -INFINITY;
-      mref[nt][u] = 0.f;
+      m[nt][u] = c_max[nt][u] = -INFINITY;
+      ref[nt][u] = 0.f;
       l[nt][u] = 0.f;
       rf[nt][u] = row_factor[nt * 8 + 2 * t + u];
     }
@@ -320,11 +322,11 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
           }
     }
     // Keys past the range stand for its last key: their scales are valid ones.
-    bool need = fmaxf(sc.z, sc.w) > vmax;
+    bool need = fmaxf(sc.z, sc.w) > vmax || !(fminf(sc.z, sc.w) >= vmax * V_LOW);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int u = 0; u < 2; u++) need |= fmaxf(x[nt][0][u], x[nt][1][u]) > m[nt][u] + M_SLACK;
+      for (int u = 0; u < 2; u++) need |= fmaxf(x[nt][0][u], x[nt][1][u]) > c_max[nt][u] + REF_SLACK;
     if (__any_sync(0xffffffffu, need)) {
       float vm = fmaxf(sc.z, sc.w);
 #pragma unroll
@@ -337,21 +339,28 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
         vmax = up;
         vinv = 1.f / up;
       }
+      const float lf = lg2(vf), lv0 = lg2(sc.z * vinv), lv1 = lg2(sc.w * vinv);
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          float tm = fmaxf(x[nt][0][u], x[nt][1][u]);
+          float mn = fmaxf(x[nt][0][u], x[nt][1][u]);
+          float cn = fmaxf(x[nt][0][u] + lv0, x[nt][1][u] + lv1);  // (a hidden key's NaN is passed over)
 #pragma unroll
-          for (int of = 4; of < 32; of <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, of));
-          const float mn = fmaxf(m[nt][u], tm);
-          const float f = m[nt][u] == -INFINITY ? 0.f : ex2(m[nt][u] - mn);
-          if (mn > m[nt][u]) {
+          for (int of = 4; of < 32; of <<= 1) {
+            mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, of));
+            cn = fmaxf(cn, __shfl_xor_sync(0xffffffffu, cn, of));
+          }
+          mn = fmaxf(mn, m[nt][u]);
+          float fo = vf;
+          if (mn > -INFINITY) {
+            c_max[nt][u] = fmaxf(c_max[nt][u] + lf, cn);
+            const float rn = weight_ref(mn, c_max[nt][u]), f = m[nt][u] == -INFINITY ? 0.f : ex2(ref[nt][u] - rn);
             l[nt][u] = l[nt][u] == 0.f ? 0.f : l[nt][u] * f;
             m[nt][u] = mn;
-            mref[nt][u] = mn - P_BIAS;
+            ref[nt][u] = rn;
+            fo *= f;
           }
-          const float fo = (mn == -INFINITY ? 1.f : f) * vf;
 #pragma unroll
           for (int k = 0; k < L::MT; k++) {
             o[nt][k][u] *= fo;
@@ -374,7 +383,7 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
 #pragma unroll
         for (int u = 0; u < 2; u++) {
           const bool ok = seen >> ((nt * 2 + k) * 2 + u) & 1;
-          const float p = ok ? ex2(x[nt][k][u] - mref[nt][u]) : 0.f;
+          const float p = ok ? ex2(x[nt][k][u] - ref[nt][u]) : 0.f;
           l[nt][u] += p;
           w[u] = ok ? p * (k ? v1 : v0) : 0.f;  // a hidden key's scale may be NaN
         }
@@ -436,7 +445,7 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
         for (int u = 0; u < 4; u++) o[nt][k][u] += ol[PS ? nt : 0][PS ? k : 0][u];
   }
 
-  // Warp states: m, l per row and O (in the values' own scale).
+  // Warp states: reference, l per row and O (in the values' own scale).
   float *so = reinterpret_cast<float *>(smem);
 #pragma unroll
   for (int nt = 0; nt < NT; nt++)
@@ -447,7 +456,7 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
       for (int of = 4; of < 32; of <<= 1) s += __shfl_xor_sync(0xffffffffu, s, of);
       const int rr = nt * 8 + 2 * t + u;
       if (g == 0) {
-        wm[warp * R + rr] = m[nt][u];
+        wm[warp * R + rr] = m[nt][u] == -INFINITY ? -INFINITY : ref[nt][u];
         wl[warp * R + rr] = s;
       }
       float *dst = so + (warp * R + rr) * D;
@@ -460,7 +469,7 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
     }
   __syncthreads();
   // A state's share of the joint one: none if it saw no key; with a NaN sum and
-  // no maximum (all its scores NaN) it passes the NaN on.
+  // no reference (all its scores NaN) it passes the NaN on.
   auto share = [](float sm, float sl, float top) {
     return sl == 0.f ? 0.f : (sm == -INFINITY ? 1.f : ex2(sm - top));
   };

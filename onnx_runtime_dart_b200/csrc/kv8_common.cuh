@@ -36,6 +36,28 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float lg2(float x) {  // -inf for 0
+  float r;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// ---- the reference of a row's weights ------------------------------------------
+// What goes to the tensor cores is w_j = 2^(x_j - ref) v_j as one or two f16 terms
+// (x_j the score in log2 units, v_j the V row's scale over the largest that the
+// kernel has met, 0 <= v_j <= 1), and l = sum 2^(x_j - ref) in fp32 beside it. f16
+// reaches from 2^-24 to 2^16, so ref has to follow the largest w_j of the row's own
+// keys, c = max (x_j + log2 v_j): taken from the scores alone, a loud V row that this
+// row does not see, or hardly weighs, would push the others' w_j out of f16 (32 keys
+// beside a hidden one 2^20 times as large: 1.7e-4 of error, 2^36: zeros). The largest
+// w_j stands at 2^REF_BIAS and may grow by 2^REF_SLACK before ref moves. The plain
+// weights are then larger than w_j by up to 1 / v_j; REF_SPAN bounds that, so that sums
+// over 2^30 keys stay below 2^120. V rows of one sequence may so differ by 2^85 before
+// the small ones of a row that sees no others lose digits. A scale not below V_LOW costs
+// none: the largest w_j is then at 2^2 or more, and what two terms cannot hold is below
+// 2^-27 of it.
+constexpr float REF_BIAS = 10.f, REF_SLACK = 5.f, REF_SPAN = 85.f, V_LOW = 0x1p-8f;
+__device__ __forceinline__ float weight_ref(float m, float c) { return fmaxf(c - REF_BIAS, m - REF_SPAN); }
 
 // Nearest e4m3 code (ties to even) of t, |t| <= 448. The hardware conversion
 // takes fp32, and rounding a double to fp32 first could land on a border that

@@ -1,0 +1,140 @@
+"""GPU tests of attention over the 8-bit KV cache where the magnitudes in one
+sequence differ: value rows that a token does not see, or hardly weighs, must
+not cost the others' digits. Each against 64 bits, and rows that do not see a
+loud value row also against the same call without it."""
+import ctypes
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+import onnx_runtime_dart_b200 as b2m  # noqa: E402
+from onnx_runtime_dart_b200 import _native as N  # noqa: E402
+from onnx_runtime_dart_b200.runtime import use_torch_stream  # noqa: E402
+from test_gpu_kv8 import Problem, _decode, _norm64, _p, _random_tree, _rope64  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = b2m.Context(0)
+    use_torch_stream(c)
+    yield c
+    c.close()
+
+
+def _mass(p):
+    """[b][s][h][d]: sum of weight times |value| over the keys each row sees, in 64 bits."""
+    q = _rope64(_norm64(p.split()[0], None if p.gain is None else p.gain[: p.h]), p.positions(), p.cos, p.sin, p.rot,
+                p.inter)
+    out = torch.zeros((p.b, p.s, p.h, p.d), dtype=torch.float64, device="cuda")
+    for i in range(p.b):
+        past = int(p.past[i])
+        n = past + p.s
+        k, v = (_decode(p.codes[x][i, :, :n], p.kv) * p.scales[x][i, :, :n].double()[..., None] for x in range(2))
+        seen = _seen(p, i)
+        for hh in range(p.h):
+            x = (q[i, :, hh] @ k[hh // (p.h // p.kvh)].T / math.sqrt(p.d)).masked_fill(~seen, -math.inf)
+            w = torch.where(seen.any(-1, keepdim=True), torch.softmax(x, -1), torch.zeros_like(x))
+            out[i, :, hh] = w @ v[hh // (p.h // p.kvh)].abs()
+    return out
+
+
+def _seen(p, i):
+    past = int(p.past[i])
+    j, t = torch.arange(past + p.s, device="cuda"), torch.arange(p.s, device="cuda")[:, None]
+    if p.tree is None:
+        return j <= past + t
+    return (j < past) | (((p.tree[i][:, None] >> (j - past).clamp(0, 63)) & 1) == 1)
+
+
+def _row_tol(p, tol):
+    """The elements' bound of Problem.answer and what a row of very different values adds: a weight times its V scale is
+    held to 2^-25 beside a largest one of 2^2 or more, 2^-27 of that, for each of n keys. (An int8 row has code 0 in some
+    dimensions: there only the quiet keys count, but the loud row's weight sets the digits. The largest weight times V
+    scale times the largest code is at most the row's largest mass.)"""
+    mass = _mass(p).amax(-1, keepdim=True).expand(p.b, p.s, p.h, p.d).reshape(tol.shape)
+    return tol + (int(p.past.max()) + p.s) * 2.0 ** -27 * mass
+
+
+HIDDEN = [  # b, s, h, kvh, d, cap, past, tree
+    (2, 3, 4, 2, 128, 80, 40, False),
+    (1, 6, 4, 2, 128, 1100, 1000, False),    # key splits over a cluster
+    (2, 7, 4, 1, 64, 100, 70, False),
+    (1, 6, 6, 2, 96, 60, 30, False),
+    (1, 5, 2, 1, 256, 60, 30, False),
+    (1, 90, 4, 2, 128, 1200, 1000, False),   # many rows, key splits
+    (2, 150, 4, 2, 64, 160, 5, False),
+    (20, 100, 8, 8, 128, 120, 10, False),    # many rows, one CTA for all keys
+    (3, 4, 4, 2, 80, 60, 30, False),         # fp32 kernel
+    (2, 12, 4, 2, 128, 100, 70, True),
+    (2, 64, 4, 2, 128, 400, 300, True),
+    (1, 60, 8, 2, 64, 64, 0, True),
+]
+
+
+@pytest.mark.parametrize("kv,loud", [("int8", 12), ("e4m3", 20), ("int8", 20), ("int8", 40), ("e4m3", 80)])
+@pytest.mark.parametrize("b,s,h,kvh,d,cap,past,tree", HIDDEN)
+def test_a_hidden_loud_value_changes_nothing(ctx, kv, loud, b, s, h, kvh, d, cap, past, tree):
+    """One new token's values 2^loud larger: rows that do not see it stay, all rows hold their bound.
+
+    Bound of the first: two calls whose weights are taken against other references. A weight's exponent is rounded once
+    at a magnitude below 2^7 (2^-18 ln 2), its exponential is off by 2^-22, its two f16 terms by 2^-22: twice these
+    are below 2^-17.2. Sums over up to 1200 keys: 76 products' additions, cut off at 2^-23 each, in either call, and
+    the weights' sum by 2^-18: below 2^-16.4 together. In all 2^-15.7 of the row's mass; an f16 row alone rounds the
+    weights to 2^-11 and the result to 2^-11 in each call."""
+    args = (kv, b, s, h, kvh, d, cap, [past] * b, 0, False, False)
+    kw = dict(tree=_random_tree(b, s, 5)) if tree else {}
+    quiet, p = Problem(*args, **kw), Problem(*args, **kw)
+    t = s // 2
+    for i in range(b):
+        p.rows[i * s + t, (h + kvh) * d:] *= 2.0 ** loud
+    outs = []
+    for prob in (quiet, p):
+        prob.attend(ctx, out=False, out16=True)
+        f16 = prob.out16.double().view(b, s, h, d)
+        prob.attend(ctx)
+        outs.append((prob.out.double().view(b, s, h, d), f16))
+    want, tol, _ = p.answer()
+    assert bool(((p.out.double() - want).abs() <= _row_tol(p, tol)).all())
+    mass = _mass(quiet)
+    for i in range(b):
+        blind = ~_seen(p, i)[:, past + t]
+        assert bool(blind.any())
+        m = mass[i, blind]
+        (a, a16), (c, c16) = ((x[i, blind] for x in o) for o in outs)
+        assert bool(((a - c).abs() <= m * 2.0 ** -15.7).all())
+        assert bool(((a16 - c16).abs() <= m * (2.0 ** -15.7 + 2 * 2.0 ** -11) + (a16.abs() + c16.abs()) * 2.0 ** -11
+                     + 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+@pytest.mark.parametrize("b,s,h,kvh,d,past", [(1, 1, 2, 1, 128, 1000), (2, 1, 8, 1, 64, 60), (1, 3, 2, 1, 128, 300),
+                                              (1, 2, 2, 1, 256, 40), (1, 90, 2, 2, 128, 700), (1, 70, 4, 2, 64, 30),
+                                              (1, 2, 2, 1, 80, 50)])
+@pytest.mark.parametrize("score,loud", [(-40.0, 24), (-40.0, 45), (-40.0, 58), (-40.0, 70), (40.0, -20), (40.0, -45),
+                                        (40.0, -70), (40.0, None)])
+def test_a_loud_value_of_no_weight(ctx, kv, b, s, h, kvh, d, past, score, loud):
+    """One cached key that every row sees, e^score times the weight of the others and with values 2^loud times as large
+    (None: zeros): against 64 bits with a bound from the weights that count."""
+    p = Problem(kv, b, s, h, kvh, d, past + s, [past] * b)
+    p.rows[:, : h * d] = 0.02
+    p.rows[:, h * d: (h + kvh) * d] = 0
+    p.codes[0].zero_()
+    p.scales[0][:, :, :past] = 1.0
+    j = past // 3
+    p.codes[0][:, :, j] = 0x40  # 64 as int8, 2 as e4m3
+    x = 0.02 * (64 if kv == "int8" else 2) * d / math.sqrt(d)
+    p.scales[0][:, :, j] = abs(score) / x
+    if score < 0:
+        p.rows[:, : h * d] *= -1
+    if loud is None:
+        p.scales[1][:, :, j] = 0
+    else:
+        p.scales[1][:, :, j] *= 2.0 ** loud
+    p.attend(ctx)
+    want, tol, _ = p.answer()
+    err, tol = (p.out.double() - want).abs(), _row_tol(p, tol)
+    assert bool((err <= tol).all()), f"{float((err / tol).max()):.2f} of the bound"
+    assert bool((p.out != 0).any())
