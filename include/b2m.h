@@ -568,12 +568,10 @@ B2M_API b2m_status b2m_kv8_read_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, co
  * h*head_dim, and / or out16, the same rounded to f16 (h*head_dim % 8 == 0);
  * one of them may be NULL. Scale <= 0 means 1/sqrt(head_dim). A token's result
  * keeps its digits whatever the value rows that it does not see, or hardly
- * weighs, hold, as long as they are below 2^85 times those that it does. With out, the
- * queries and the softmax weights are split into two f16 terms on the tensor
- * cores (about 1e-6 of the largest value of a row, 2.4e-6 over thousands of
- * keys). With out16 alone one of the two is rounded to f16 once (the weights
- * for calls of few query rows per kv head, the queries for many): an error
- * like that of the output's own rounding. EXACT attention mode (b2m_set_attention_mode) runs
+ * weighs, hold, as long as they are below 2^85 times those that it does. The queries
+ * and the softmax weights are split into two f16 terms on the tensor cores
+ * (about 1e-6 of the largest value of a row, 2.4e-6 over thousands of keys);
+ * out16 holds the same rows rounded once, with or without out. EXACT attention mode (b2m_set_attention_mode) runs
  * the fp32 CUDA-core kernel. */
 B2M_API b2m_status b2m_gqa_kv8_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const float *q, const float *k,
                                    const float *v, int64_t q_rs, int64_t kv_rs, const float *qk_gain, double eps,

@@ -21,10 +21,9 @@
 // No cross-thread reduction is left in the softmax. Two CTAs share an SM, so one's
 // exponentials run under the other's products.
 //
-// P is split into two f16 terms (22 bits, two products); so is Q (QS) where fp32
-// rows are wanted. For an f16 output alone Q is rounded to f16 once: an error like
-// that of the output's own rounding (against 64 bits 2.8e-4 in all, 2.1e-4 with
-// both split, 3.5e-4 with neither; 259, 281 and 250 us for 4 x 2048 tokens).
+// Q and P are split into two f16 terms (22 bits, two products each), for an f16
+// output too: with one term of Q its error against 64 bits was 2.8e-4, the output's own
+// rounding is 2.1e-4.
 //
 // Few row tiles over many keys (a tree on long sequences): the CTAs of a cluster
 // split the keys and merge their O, reference and l through distributed shared memory in
@@ -146,14 +145,13 @@ __device__ __forceinline__ bool warp_wait_phase(uint64_t *bar, uint32_t parity, 
   return __all_sync(0xffffffffu, wait_phase(bar, parity, abort_flag, dev_err));
 }
 
-template <int D, bool QS>
+template <int D>
 struct FlashLayout {
   static constexpr int ND = D / 64;
-  static constexpr int KST = QS ? 1 : 2, VST = QS ? 1 : 2;
   static constexpr uint32_t QH = 0, QL = ND * 16384;
-  static constexpr uint32_t K = QL + (QS ? ND * 16384 : 0), K_STAGE = ND * 8192;
-  static constexpr uint32_t V = K + KST * K_STAGE, V_STAGE = D * 128;
-  static constexpr uint32_t TILES = V + VST * V_STAGE;
+  static constexpr uint32_t K = QL + ND * 16384;  // one K and one V tile (two of each are more than half of an SM's memory)
+  static constexpr uint32_t V = K + ND * 8192;
+  static constexpr uint32_t TILES = V + D * 128;
   // O staging [128][D + 4] fp32 at the end, over Q, K and V
   static constexpr int OST = D + 4;
   static constexpr uint32_t SCALES0 = 128 * OST * 4 > TILES ? 128 * OST * 4 : TILES;
@@ -163,15 +161,15 @@ struct FlashLayout {
   static constexpr uint32_t VF = SCALES + FL_SLOTS * 64 * 8, VFLAG = VF + FL_SLOTS * 4, VREF = VFLAG + FL_SLOTS * 4;
   static constexpr uint32_t ROWS = VREF + 16;
   static constexpr uint32_t BARS = ROWS + 128 * (8 + 4 + 4 + 4 + 4);
-  static constexpr uint32_t SLOT = BARS + 14 * 8, FLAG = SLOT + 4;
+  static constexpr uint32_t SLOT = BARS + 10 * 8, FLAG = SLOT + 4;
   static constexpr uint32_t BYTES = FLAG + 4;
   static constexpr uint32_t T_O = 128;  // TMEM: S / P buffers at 0 and 64, O at 128
   static_assert(BYTES <= 113 * 1024, "two CTAs per SM");
 };
 
-template <bool E4M3, int D, bool QS, bool PS>
+template <bool E4M3, int D>
 __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args a) {
-  using L = FlashLayout<D, QS>;
+  using L = FlashLayout<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
   float *ks_s = reinterpret_cast<float *>(smem + L::SCALES), *vs_s = ks_s + FL_SLOTS * 64;
   float *vf_s = reinterpret_cast<float *>(smem + L::VF), *vref_s = reinterpret_cast<float *>(smem + L::VREF);
@@ -181,8 +179,8 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   int *row_lim = reinterpret_cast<int *>(row_factor + 128);
   float *row_ref = reinterpret_cast<float *>(row_lim + 128), *row_l = row_ref + 128;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BARS);
-  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8,
-           *p_full = bars + 10, *o_done = bars + 12, *all_done = bars + 13;
+  uint64_t *k_full = bars, *k_empty = bars + 1, *v_full = bars + 2, *v_empty = bars + 3, *s_full = bars + 4,
+           *p_full = bars + 6, *o_done = bars + 8, *all_done = bars + 9;
   uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::SLOT);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::FLAG);
 
@@ -200,11 +198,11 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
   const int64_t base = ((int64_t)b * a.KVH + kvh) * a.CAP;
 
   if (tid == 0) {
+    mbar_init(k_full, 128);
+    mbar_init(k_empty, 1);
+    mbar_init(v_full, 128);
+    mbar_init(v_empty, 1);
     for (int i = 0; i < 2; i++) {
-      mbar_init(k_full + i, 128);
-      mbar_init(k_empty + i, 1);
-      mbar_init(v_full + i, 128);
-      mbar_init(v_empty + i, 1);
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 128);
     }
@@ -239,12 +237,9 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
         const uint32_t at = (uint32_t)(d >> 6) * 16384u + sw128(rr, d & 63);
         *reinterpret_cast<uint2 *>(smem + L::QH + at) = make_uint2(h2_as_u32(h0), h2_as_u32(h1));
-        if (QS) {
-          const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
-          *reinterpret_cast<uint2 *>(smem + L::QL + at) =
-              make_uint2(h2_as_u32(__floats2half2_rn(x.x - g0.x, x.y - g0.y)),
-                         h2_as_u32(__floats2half2_rn(x.z - g1.x, x.w - g1.y)));
-        }
+        const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
+        *reinterpret_cast<uint2 *>(smem + L::QL + at) = make_uint2(
+            h2_as_u32(__floats2half2_rn(x.x - g0.x, x.y - g0.y)), h2_as_u32(__floats2half2_rn(x.z - g1.x, x.w - g1.y)));
       }
       if ((lane & 7) == 0) {
         row_factor[rr] = q.factor;
@@ -298,10 +293,9 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     };
     float vref = 0.f, vinv = 0.f;
     auto put_k = [&](int t) {
-      const int kst = t % L::KST, sl = t % FL_SLOTS;
-      if (t >= L::KST && !warp_wait_phase(k_empty + kst, (uint32_t)(t / L::KST - 1) & 1u, abort_flag, a.err))
-        return false;
-      uint8_t *kd = smem + L::K + kst * L::K_STAGE;
+      const int sl = t % FL_SLOTS;
+      if (t > 0 && !warp_wait_phase(k_empty, (uint32_t)(t - 1) & 1u, abort_flag, a.err)) return false;
+      uint8_t *kd = smem + L::K;
 #pragma unroll
       for (int u = 0; u < KI; u++) {
         int row, c;
@@ -342,7 +336,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         }
       }
       fence_proxy_async_smem();
-      mbar_arrive(k_full + kst);
+      mbar_arrive(k_full);
       return true;
     };
     // The append of the call's rows may still run: tiles without new rows go ahead
@@ -374,9 +368,8 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           load_k(t + 2);
         }
       }
-      const int vst = t % L::VST;
-      if (t >= L::VST && !warp_wait_phase(v_empty + vst, (uint32_t)(t / L::VST - 1) & 1u, abort_flag, a.err)) break;
-      uint8_t *vd = smem + L::V + vst * L::V_STAGE;
+      if (t > 0 && !warp_wait_phase(v_empty, (uint32_t)(t - 1) & 1u, abort_flag, a.err)) break;
+      uint8_t *vd = smem + L::V;
 #pragma unroll
       for (int u = 0; u < VI; u++) {
         const uint32_t w0[4] = {vreg[0][u].x, vreg[0][u].y, vreg[0][u].z, vreg[0][u].w};
@@ -391,7 +384,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         }
       }
       fence_proxy_async_smem();
-      mbar_arrive(v_full + vst);
+      mbar_arrive(v_full);
       if (t + 1 < ntile) load_v(t + 1);
     }
   } else if (warp >= 8) {
@@ -402,19 +395,19 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
       const uint32_t sb = smem_u32(smem);
       const uint64_t d_qh = sw128_kmajor_desc(sb + L::QH), d_ql = sw128_kmajor_desc(sb + L::QL);
       auto issue_s = [&](int t) {
-        const uint64_t dk = sw128_kmajor_desc(sb + L::K + (t % L::KST) * L::K_STAGE);
+        const uint64_t dk = sw128_kmajor_desc(sb + L::K);
         const uint32_t ts = tmem + (uint32_t)(t & 1) * 64u;
         // the lower terms first: fewer additions to a sum of full size
 #pragma unroll
-        for (int part = QS ? 0 : 1; part < 2; part++)
+        for (int part = 0; part < 2; part++)
 #pragma unroll
           for (int kk = 0; kk < D / 16; kk++) {
             const uint64_t oq = ((kk >> 2) * 16384u + (kk & 3) * 32u) >> 4,
                            ok = ((kk >> 2) * 8192u + (kk & 3) * 32u) >> 4;
-            umma_f16(ts, (part ? d_qh : d_ql) + oq, dk + ok, idesc_s, (QS && part) || kk ? 1u : 0u);
+            umma_f16(ts, (part ? d_qh : d_ql) + oq, dk + ok, idesc_s, part || kk ? 1u : 0u);
           }
         umma_commit(s_full + (t & 1));
-        umma_commit(k_empty + t % L::KST);
+        umma_commit(k_empty);
       };
       bool ok = wait_phase(k_full, 0u, abort_flag, a.err);
       if (ok) {
@@ -424,28 +417,27 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
 #pragma unroll 1
       for (int t = 0; ok && t < ntile; t++) {
         if (t + 1 < ntile) {
-          const int st = (t + 1) % L::KST;
           // S_{t+1} takes the columns of P_{t-1}: products of different shapes are
           // not ordered among themselves, so P_{t-1} . V must be through.
           ok = (t == 0 || wait_phase(o_done, (uint32_t)(t - 1) & 1u, abort_flag, a.err)) &&
-               wait_phase(k_full + st, (uint32_t)((t + 1) / L::KST) & 1u, abort_flag, a.err);
+               wait_phase(k_full, (uint32_t)(t + 1) & 1u, abort_flag, a.err);
           if (!ok) break;
           tc_fence_after();
           issue_s(t + 1);
         }
-        ok = wait_phase(v_full + t % L::VST, (uint32_t)(t / L::VST) & 1u, abort_flag, a.err) &&
+        ok = wait_phase(v_full, (uint32_t)t & 1u, abort_flag, a.err) &&
              wait_phase(p_full + (t & 1), (uint32_t)(t >> 1) & 1u, abort_flag, a.err);
         if (!ok) break;
         tc_fence_after();
-        const uint64_t dv = sw128_kmajor_desc(sb + L::V + (t % L::VST) * L::V_STAGE);
+        const uint64_t dv = sw128_kmajor_desc(sb + L::V);
         const uint32_t tp = tmem + (uint32_t)(t & 1) * 64u;
 #pragma unroll
-        for (int part = PS ? 0 : 1; part < 2; part++)
+        for (int part = 0; part < 2; part++)
 #pragma unroll
           for (int kk = 0; kk < FL_TILE / 16; kk++)
             umma_f16_ts(tmem + L::T_O, tp + (part ? 0u : 32u) + 8u * kk, dv + ((kk * 32u) >> 4), idesc_o,
-                        t || (PS && part) || kk ? 1u : 0u);
-        umma_commit(v_empty + t % L::VST);
+                        t || part || kk ? 1u : 0u);
+        umma_commit(v_empty);
         umma_commit(o_done);
         // A barrier of its own for the last one: a waiter that has not seen the
         // phase before could take o_done's parity for the one it waits for. (In the
@@ -572,7 +564,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         }
       }
       const f32x2 rf2 = pack2(rf, rf), mr2 = pack2(-ref, -ref);
-      uint32_t ph[32], pl[PS ? 32 : 1];
+      uint32_t ph[32], pl[32];
       f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < FL_TILE / 4; c++) {
@@ -587,10 +579,8 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           unpack2(mul2(p, k ? v4.y : v4.x), w0, w1);
           const __half2 h = __floats2half2_rn(w0, w1);
           ph[2 * c + k] = h2_as_u32(h);
-          if (PS) {
-            const float2 g = __half22float2(h);
-            pl[PS ? 2 * c + k : 0] = h2_as_u32(__floats2half2_rn(w0 - g.x, w1 - g.y));
-          }
+          const float2 g = __half22float2(h);
+          pl[2 * c + k] = h2_as_u32(__floats2half2_rn(w0 - g.x, w1 - g.y));
         }
       }
       if ((vflag & 1) && !whole) {
@@ -601,7 +591,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           const uint32_t w = c < 16 ? s0 : s1;
           const uint32_t keep = (w >> (2 * c & 31) & 1 ? 0xffffu : 0u) | (w >> (2 * c + 1 & 31) & 1 ? 0xffff0000u : 0u);
           ph[c] &= keep;
-          if (PS) pl[PS ? c : 0] &= keep;
+          pl[c] &= keep;
         }
       }
       {
@@ -611,7 +601,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
         l += (a0 + a1) + (b0 + b1);
       }
       tmem_st32(ts, ph);
-      if constexpr (PS) tmem_st32(ts + 32u, pl);
+      tmem_st32(ts + 32u, pl);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(p_full + (t & 1));  // two: a warp may be a tile ahead of another (S_{t+1} is there early)
@@ -731,10 +721,10 @@ void require_regs_once() {
               "GroupQueryAttention (8-bit cache): the flash kernel was built with another register count");
 }
 
-template <bool E4M3, int D, bool QS, bool PS>
+template <bool E4M3, int D>
 void launch(const Kv8Args &a, cudaStream_t s) {
-  using L = FlashLayout<D, QS>;
-  constexpr auto kern = kv8_flash_kernel<E4M3, D, QS, PS>;
+  using L = FlashLayout<D>;
+  constexpr auto kern = kv8_flash_kernel<E4M3, D>;
   set_smem_limit_once<kern>((int)L::BYTES);
   require_regs_once<kern>();
   const int nrows = a.S * (a.H / a.KVH), tiles = (nrows + FL_ROWS - 1) / FL_ROWS;
@@ -762,14 +752,6 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   B2M_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
 }
 
-template <bool E4M3, int D>
-void launch_out(const Kv8Args &a, cudaStream_t s) {
-  if (a.out)
-    launch<E4M3, D, true, true>(a, s);
-  else
-    launch<E4M3, D, false, true>(a, s);
-}
-
 }  // namespace
 
 // Enough rows, head dims and alignments the kernel takes. The other kernel reads
@@ -789,13 +771,13 @@ bool kv8_flash_shape(const Kv8Args &a) {
 void launch_kv8_flash(const Kv8Args &a, cudaStream_t s) {
   if (a.e4m3) {
     if (a.D == 128)
-      launch_out<true, 128>(a, s);
+      launch<true, 128>(a, s);
     else
-      launch_out<true, 64>(a, s);
+      launch<true, 64>(a, s);
   } else {
     if (a.D == 128)
-      launch_out<false, 128>(a, s);
+      launch<false, 128>(a, s);
     else
-      launch_out<false, 64>(a, s);
+      launch<false, 64>(a, s);
   }
 }

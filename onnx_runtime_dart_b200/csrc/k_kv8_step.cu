@@ -8,10 +8,9 @@
 //   S^T[16 keys][8 rows] = K . Q^T,   O^T[D][8 rows] += V^T . P^T.
 // The codes are the A operands: int8 and e4m3 codes are f16 numbers exactly, so
 // they are expanded in registers and the scales applied in fp32, K's to the
-// scores and V's to the weights. Q and (PS: fp32 rows are wanted) the weights are
-// split into two f16 terms (22 bits), so the products carry fp32 accuracy; for an
-// f16 output alone the weights are rounded to f16 once, an error like that of the
-// output's own rounding. Which D index or key an MMA
+// scores and V's to the weights. Q and the weights are split into two f16 terms (22
+// bits), so the products carry fp32 accuracy, for an f16 output too (one term of the
+// weights would put 2.9e-4 of error where the output's own rounding is 2.1e-4). Which D index or key an MMA
 // lane holds is free as long as both operands agree: lanes are given 16
 // consecutive bytes of a row, so no data is shuffled on its way to the tensor
 // cores; only P^T is transposed between the two products (movmatrix).
@@ -98,7 +97,7 @@ struct StepSmem {
 
 // (The CTAs per SM that the registers allow anyway, said to the compiler: 32 trees
 // of 8 tokens 42 us, 45 .. 47 without.)
-template <bool E4M3, int D, int NT, bool PS>
+template <bool E4M3, int D, int NT>
 __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
     kv8_step_kernel(const Kv8Args a, const int fused_append) {
   using L = StepShape<D>;
@@ -222,10 +221,10 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
       if (k >= ahead) issue(warp + k * ST_WARPS, k);
   }
 
-  // With PS the products of the lower terms have sums of their own: the tensor
-  // cores cut off what an addition to a sum leaves below it, always toward zero,
-  // and half as many additions to the large sums halve that.
-  float o[NT][L::MT][4], ol[PS ? NT : 1][PS ? L::MT : 1][4];
+  // The products of the lower terms have sums of their own: the tensor cores cut off
+  // what an addition to a sum leaves below it, always toward zero, and half as many
+  // additions to the large sums halve that.
+  float o[NT][L::MT][4], ol[NT][L::MT][4];
   // Per row: the largest score seen, log2 of the largest weight times V scale (at
   // reference weight 1), the reference, the weights' sum, the scores' factor.
   float m[NT][2], c_max[NT][2], ref[NT][2], l[NT][2], rf[NT][2];
@@ -234,10 +233,7 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
 #pragma unroll
     for (int k = 0; k < L::MT; k++)
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        o[nt][k][u] = 0.f;
-        if (PS) ol[PS ? nt : 0][PS ? k : 0][u] = 0.f;
-      }
+      for (int u = 0; u < 4; u++) o[nt][k][u] = ol[nt][k][u] = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       m[nt][u] = c_max[nt][u] = -INFINITY;
@@ -365,10 +361,8 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
           for (int k = 0; k < L::MT; k++) {
             o[nt][k][u] *= fo;
             o[nt][k][2 + u] *= fo;
-            if (PS) {
-              ol[PS ? nt : 0][PS ? k : 0][u] *= fo;
-              ol[PS ? nt : 0][PS ? k : 0][2 + u] *= fo;
-            }
+            ol[nt][k][u] *= fo;
+            ol[nt][k][2 + u] *= fo;
           }
         }
     }
@@ -389,10 +383,8 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
         }
         const __half2 h = __floats2half2_rn(w[0], w[1]);
         bh[nt][k] = transpose8x8(b2m::h2_as_u32(h));
-        if (PS) {
-          const float2 hf = __half22float2(h);
-          bl[nt][k] = transpose8x8(b2m::h2_as_u32(__floats2half2_rn(w[0] - hf.x, w[1] - hf.y)));
-        }
+        const float2 hf = __half22float2(h);
+        bl[nt][k] = transpose8x8(b2m::h2_as_u32(__floats2half2_rn(w[0] - hf.x, w[1] - hf.y)));
       }
     // O^T += V^T . P^T
 #pragma unroll
@@ -421,13 +413,10 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
         for (int hf = 0; hf < 2; hf++)
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) mma(o[nt][(cc * L::VW + w) * 2 + hf], A[hf], bh[nt][0], bh[nt][1]);
-        if (PS) {
 #pragma unroll
-          for (int hf = 0; hf < 2; hf++)
+        for (int hf = 0; hf < 2; hf++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-              mma(ol[PS ? nt : 0][PS ? (cc * L::VW + w) * 2 + hf : 0], A[hf], bl[nt][0], bl[nt][1]);
-        }
+          for (int nt = 0; nt < NT; nt++) mma(ol[nt][(cc * L::VW + w) * 2 + hf], A[hf], bl[nt][0], bl[nt][1]);
       }
     }
     slot = slot + 1 == ST_STAGES ? 0 : slot + 1;
@@ -436,14 +425,12 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
   cp_wait<0>();
   __syncthreads();  // the rings are drained: the states reuse them
 
-  if (PS) {
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+  for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int k = 0; k < L::MT; k++)
+    for (int k = 0; k < L::MT; k++)
 #pragma unroll
-        for (int u = 0; u < 4; u++) o[nt][k][u] += ol[PS ? nt : 0][PS ? k : 0][u];
-  }
+      for (int u = 0; u < 4; u++) o[nt][k][u] += ol[nt][k][u];
 
   // Warp states: reference, l per row and O (in the values' own scale).
   float *so = reinterpret_cast<float *>(smem);
@@ -542,10 +529,10 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
   if (CL > 1) cluster.sync();  // the others have read this CTA's state
 }
 
-template <bool E4M3, int D, int NT, bool PS>
+template <bool E4M3, int D, int NT>
 void launch(const Kv8Args &a, cudaStream_t s) {
   using M = StepSmem<D, NT>;
-  constexpr auto kern = kv8_step_kernel<E4M3, D, NT, PS>;
+  constexpr auto kern = kv8_step_kernel<E4M3, D, NT>;
   b2m::set_smem_limit_once<kern>(M::BYTES);
   const int nrows = a.S * (a.H / a.KVH), tiles = (nrows + M::R - 1) / M::R;
   // One new row per sequence is appended beside the query rows; more would hold up
@@ -583,20 +570,12 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   B2M_CUDA(cudaLaunchKernelEx(&cfg, kern, a, fused ? 1 : 0));
 }
 
-template <bool E4M3, int D, int NT>
-void launch_out(const Kv8Args &a, cudaStream_t s) {
-  if (a.out)
-    launch<E4M3, D, NT, true>(a, s);
-  else
-    launch<E4M3, D, NT, false>(a, s);
-}
-
 template <bool E4M3, int D>
 void launch_rows(const Kv8Args &a, cudaStream_t s) {
   if (a.S * (a.H / a.KVH) <= 8)
-    launch_out<E4M3, D, 1>(a, s);
+    launch<E4M3, D, 1>(a, s);
   else
-    launch_out<E4M3, D, 2>(a, s);
+    launch<E4M3, D, 2>(a, s);
 }
 
 template <bool E4M3>
@@ -606,7 +585,7 @@ void launch_dim(const Kv8Args &a, cudaStream_t s) {
     case 64: return launch_rows<E4M3, 64>(a, s);
     case 96: return launch_rows<E4M3, 96>(a, s);
     case 128: return launch_rows<E4M3, 128>(a, s);
-    default: return launch_out<E4M3, 256, 1>(a, s);
+    default: return launch<E4M3, 256, 1>(a, s);
   }
 }
 

@@ -138,3 +138,17 @@ def test_a_loud_value_of_no_weight(ctx, kv, b, s, h, kvh, d, past, score, loud):
     err, tol = (p.out.double() - want).abs(), _row_tol(p, tol)
     assert bool((err <= tol).all()), f"{float((err / tol).max()):.2f} of the bound"
     assert bool((p.out != 0).any())
+
+
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+@pytest.mark.parametrize("b,s,h,kvh,d,cap,past", [(2, 1, 4, 2, 128, 700, 600), (1, 1, 16, 1, 64, 90, 50),
+                                                  (2, 5, 4, 2, 96, 60, 30), (1, 3, 2, 2, 256, 40, 20),
+                                                  (2, 1, 3, 1, 32, 300, 290), (2, 90, 4, 2, 128, 400, 300),
+                                                  (8, 64, 32, 8, 64, 80, 10), (1, 4, 4, 2, 80, 40, 9)])
+def test_f16_rows_are_the_fp32_rows_rounded(ctx, kv, b, s, h, kvh, d, cap, past):
+    """An f16 output alone is computed as the fp32 rows are: the same bits as rounding those."""
+    p = Problem(kv, b, s, h, kvh, d, cap, [past] * b, d, False, True)
+    p.attend(ctx)
+    full = p.out.clone()
+    p.attend(ctx, out=False, out16=True)
+    assert torch.equal(p.out16, full.half())
