@@ -570,7 +570,7 @@ B2M_API b2m_status b2m_kv8_read_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, co
  * keeps its digits whatever the value rows that it does not see, or hardly
  * weighs, hold, as long as they are below 2^85 times those that it does. The queries
  * and the softmax weights are split into two f16 terms on the tensor cores
- * (about 1e-6 of the largest value of a row, 2.4e-6 over thousands of keys);
+ * (about 1e-6 of the largest value of a row, however many keys it sees);
  * out16 holds the same rows rounded once, with or without out. EXACT attention mode (b2m_set_attention_mode) runs
  * the fp32 CUDA-core kernel. */
 B2M_API b2m_status b2m_gqa_kv8_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const float *q, const float *k,

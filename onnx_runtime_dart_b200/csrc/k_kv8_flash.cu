@@ -51,7 +51,8 @@ namespace cg = cooperative_groups;
 using namespace kv8;
 using namespace b2m;
 
-constexpr int FL_MAX_CLUSTER = 8, FL_THREADS = 384, FL_TILE = 64, FL_ROWS = 128, FL_SLOTS = 4;
+constexpr int FL_MAX_CLUSTER = 8, FL_THREADS = 384, FL_TILE = 64, FL_ROWS = 128, FL_SLOTS = 4,
+              FL_WINDOW = 8;  // tiles whose products the tensor cores add up (see the softmax's totals)
 // Registers per thread: at launch (two CTAs per SM), then per role, and the
 // launch's number again for the common end. The CTA's three warpgroups share
 // what it was launched with: the roles' sum is no more.
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
 #pragma unroll
           for (int kk = 0; kk < FL_TILE / 16; kk++)
             umma_f16_ts(tmem + L::T_O, tp + (part ? 0u : 32u) + 8u * kk, dv + ((kk * 32u) >> 4), idesc_o,
-                        t || part || kk ? 1u : 0u);
+                        t % FL_WINDOW || part || kk ? 1u : 0u);
         umma_commit(v_empty);
         umma_commit(o_done);
         // A barrier of its own for the last one: a waiter that has not seen the
@@ -457,13 +458,63 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     // Largest score seen, log2 of the largest weight times V scale (at the reference
     // weight 1), the reference the weights are taken against, their sum.
     float m = -INFINITY, c_max = -INFINITY, ref = 0.f, l = 0.f;
+    // The tensor cores cut off what an addition to O leaves below it, always toward
+    // zero: eight times per tile, 1.6e-7 of a sum of equal signs (1e-5 after 60 tiles,
+    // without a bound as sequences grow). So O starts anew every FL_WINDOW tiles, and
+    // the row's thread adds what it held, rounded to nearest, to totals of its own:
+    // thread-local memory, which is laid out across a warp's threads and mostly stays
+    // in L2. `carry` is what the totals are to be multiplied by since the last time.
+    alignas(16) float total[D];
+    float carry = 1.f;
+    // Waits for phase `parity` of `done`, then calls put(d, totals + O of dimensions d ..
+    // d + 3) for all of them; 64 totals at a time are requested ahead (as long a way as
+    // a tile's products take).
+    auto with_totals = [&](bool any, uint64_t *done, uint32_t parity, auto put) {
+      float4 held[16];
+      int d0 = 0;
+      asm volatile("" : "+r"(d0));  // (an index the compiler knows would put the totals into registers that are not there)
+      auto fetch = [&](int d) {
+#pragma unroll
+        for (int k = 0; k < 16; k++)
+          held[k] = any ? reinterpret_cast<const float4 *>(total + d)[k] : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      fetch(d0);
+      if (!warp_wait_phase(done, parity, abort_flag, a.err)) return false;
+      tc_fence_after();
+#pragma unroll 1
+      for (int d = d0; d < D; d += 64) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          uint32_t u[16];
+          tmem_ld16(trow + L::T_O + d + 16u * q, u);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const float4 v = held[4 * q + k];
+            put(d + 16 * q + 4 * k, make_float4(fmaf(v.x, carry, __uint_as_float(u[4 * k])),
+                                                fmaf(v.y, carry, __uint_as_float(u[4 * k + 1])),
+                                                fmaf(v.z, carry, __uint_as_float(u[4 * k + 2])),
+                                                fmaf(v.w, carry, __uint_as_float(u[4 * k + 3]))));
+          }
+        }
+        if (d + 64 < D) fetch(d + 64);
+      }
+      return true;
+    };
     bool ok = true;
 #pragma unroll 1
     for (int t = 0; t < ntile; t++) {
+      const bool anew = t % FL_WINDOW == 0;
       const int sl = t % FL_SLOTS, j0 = (t0 + t) * FL_TILE;
       ok = warp_wait_phase(s_full + (t & 1), (uint32_t)(t >> 1) & 1u, abort_flag, a.err);
       if (!ok) break;
       tc_fence_after();
+      if (anew && t > 0) {
+        ok = with_totals(t > FL_WINDOW, o_done, (uint32_t)(t - 1) & 1u,
+                         [&](int d, const float4 &v) { *reinterpret_cast<float4 *>(total + d) = v; });
+        if (!ok) break;
+        carry = 1.f;
+      }
       const uint32_t ts = trow + (uint32_t)(t & 1) * 64u;
       // Scores of the row's 64 keys as 32 pairs, times K's scales.
       f32x2 x[FL_TILE / 2];
@@ -541,7 +592,8 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
           m = mn;
           ref = rn;
         }
-        if (t > 0) {  // O holds the tiles before: rescale it once their products are done
+        carry *= f;
+        if (!anew) {  // O holds the tiles before: rescale it once their products are done
           ok = warp_wait_phase(o_done, (uint32_t)(t - 1) & 1u, abort_flag, a.err);
           if (!ok) break;
           tc_fence_after();
@@ -606,28 +658,19 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
       tc_fence_before();
       mbar_arrive(p_full + (t & 1));  // two: a warp may be a tile ahead of another (S_{t+1} is there early)
     }
-    if (ok && ntile > 0) ok = warp_wait_phase(all_done, 0u, abort_flag, a.err);
-    tc_fence_after();
     // O (in the values' own scale), reference and l to shared memory: Q, K and V are no
     // longer read (the last products have completed).
     float *ost = reinterpret_cast<float *>(smem) + rr * L::OST;
-    if (ok) {
+    if (ok && ntile > 0) {
       // (alone, a CTA divides here; a row that saw nothing: zeros)
-      const float vo = ntile == 0 ? 0.f : (CL > 1 ? *vref_s : (l == 0.f ? 0.f : *vref_s / l));
-#pragma unroll
-      for (int c = 0; c < D / 16; c++) {
-        uint32_t u[16];
-        if (ntile > 0) {
-          tmem_ld16(trow + L::T_O + 16u * c, u);
-          tmem_ld_wait();
-        }
-#pragma unroll
-        for (int k = 0; k < 16; k += 4)
-          *reinterpret_cast<float4 *>(ost + 16 * c + k) =
-              ntile > 0 ? make_float4(__uint_as_float(u[k]) * vo, __uint_as_float(u[k + 1]) * vo,
-                                      __uint_as_float(u[k + 2]) * vo, __uint_as_float(u[k + 3]) * vo)
-                        : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+      float vo = 0.f;
+      ok = with_totals(ntile > FL_WINDOW, all_done, 0u, [&](int d, const float4 &v) {
+        if (d == 0) vo = CL > 1 ? *vref_s : (l == 0.f ? 0.f : *vref_s / l);
+        *reinterpret_cast<float4 *>(ost + d) = make_float4(v.x * vo, v.y * vo, v.z * vo, v.w * vo);
+      });
+    } else if (ok) {
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4) *reinterpret_cast<float4 *>(ost + d) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     row_ref[rr] = m == -INFINITY ? -INFINITY : ref;
     row_l[rr] = l;

@@ -42,7 +42,7 @@ namespace {
 namespace cg = cooperative_groups;
 using namespace kv8;
 
-constexpr int ST_WARPS = 4, ST_THREADS = 32 * ST_WARPS, ST_STAGES = 3;
+constexpr int ST_WARPS = 4, ST_THREADS = 32 * ST_WARPS, ST_STAGES = 3, ST_WINDOW = 16;
 
 template <int N>
 __device__ __forceinline__ void cp_async(void *dst, const void *src) {
@@ -221,10 +221,10 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
       if (k >= ahead) issue(warp + k * ST_WARPS, k);
   }
 
-  // The products of the lower terms have sums of their own: the tensor cores cut off
-  // what an addition to a sum leaves below it, always toward zero, and half as many
-  // additions to the large sums halve that.
-  float o[NT][L::MT][4], ol[NT][L::MT][4];
+  // The tensor cores cut off what an addition to a sum leaves below it, always toward
+  // zero: over n additions some n 2^-25 of the sum. So they only sum ST_WINDOW tiles,
+  // which are then added, rounded to nearest, to the totals.
+  float o[NT][L::MT][4], total[NT][L::MT][4];
   // Per row: the largest score seen, log2 of the largest weight times V scale (at
   // reference weight 1), the reference, the weights' sum, the scores' factor.
   float m[NT][2], c_max[NT][2], ref[NT][2], l[NT][2], rf[NT][2];
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
 #pragma unroll
     for (int k = 0; k < L::MT; k++)
 #pragma unroll
-      for (int u = 0; u < 4; u++) o[nt][k][u] = ol[nt][k][u] = 0.f;
+      for (int u = 0; u < 4; u++) o[nt][k][u] = total[nt][k][u] = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       m[nt][u] = c_max[nt][u] = -INFINITY;
@@ -245,7 +245,19 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
   float vmax = 0.f, vinv = 0.f;  // largest V scale seen (a power of two above it), and its reciprocal
   const int all_see = a.tree ? past : past + row0 / G + 1;  // keys below this are seen by every row
 
-  int slot = 0;
+  auto fold = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int k = 0; k < L::MT; k++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          total[nt][k][u] += o[nt][k][u];
+          o[nt][k][u] = 0.f;
+        }
+  };
+
+  int slot = 0, window = 0;
 #pragma unroll 1
   for (int tile = warp; tile < ntile; tile += ST_WARPS) {
     cp_wait<ST_STAGES - 2>();
@@ -361,8 +373,8 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
           for (int k = 0; k < L::MT; k++) {
             o[nt][k][u] *= fo;
             o[nt][k][2 + u] *= fo;
-            ol[nt][k][u] *= fo;
-            ol[nt][k][2 + u] *= fo;
+            total[nt][k][u] *= fo;
+            total[nt][k][2 + u] *= fo;
           }
         }
     }
@@ -416,8 +428,12 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
 #pragma unroll
         for (int hf = 0; hf < 2; hf++)
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) mma(ol[nt][(cc * L::VW + w) * 2 + hf], A[hf], bl[nt][0], bl[nt][1]);
+          for (int nt = 0; nt < NT; nt++) mma(o[nt][(cc * L::VW + w) * 2 + hf], A[hf], bl[nt][0], bl[nt][1]);
       }
+    }
+    if (++window == ST_WINDOW) {
+      window = 0;
+      fold();
     }
     slot = slot + 1 == ST_STAGES ? 0 : slot + 1;
     __syncwarp();  // every lane has read the slot's scales before it is refilled
@@ -425,12 +441,7 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
   cp_wait<0>();
   __syncthreads();  // the rings are drained: the states reuse them
 
-#pragma unroll
-  for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-    for (int k = 0; k < L::MT; k++)
-#pragma unroll
-      for (int u = 0; u < 4; u++) o[nt][k][u] += ol[nt][k][u];
+  fold();
 
   // Warp states: reference, l per row and O (in the values' own scale).
   float *so = reinterpret_cast<float *>(smem);
@@ -451,7 +462,7 @@ __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
       for (int k = 0; k < L::MT; k++) {
         const int cc = (k >> 1) / L::VW, w = (k >> 1) % L::VW;
         const int d = (cc * 8 + g) * L::VC + 4 * w + 2 * (k & 1);
-        *reinterpret_cast<float2 *>(dst + d) = make_float2(o[nt][k][u] * vmax, o[nt][k][2 + u] * vmax);
+        *reinterpret_cast<float2 *>(dst + d) = make_float2(total[nt][k][u] * vmax, total[nt][k][2 + u] * vmax);
       }
     }
   __syncthreads();

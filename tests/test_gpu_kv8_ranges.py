@@ -152,3 +152,34 @@ def test_f16_rows_are_the_fp32_rows_rounded(ctx, kv, b, s, h, kvh, d, cap, past)
     full = p.out.clone()
     p.attend(ctx, out=False, out16=True)
     assert torch.equal(p.out16, full.half())
+
+
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+@pytest.mark.parametrize("b,s,h,kvh,d,n", [
+    (19, 64, 16, 8, 128, 16384),  # one CTA for all keys of 128 query rows
+    (19, 64, 16, 8, 64, 16000),
+    (28, 1, 16, 8, 128, 32768),   # one CTA, four warps, for all keys of a few rows
+    (28, 1, 16, 8, 64, 32760),
+    (28, 6, 16, 8, 64, 16384)])
+def test_sums_do_not_drift(ctx, kv, b, s, h, kvh, d, n):
+    """Equal scores and equal values: each output is the value itself, however many keys there are.
+
+    All weights are 2^10 and their sum is exact. What the tensor cores cut off an addition is below 2^-23 of the sum so
+    far: over a window of 64 additions (eight tiles, four steps, two terms) 32 * 2^-23 of the window, less where a window
+    has 16. At most 64 windows are added up, each rounded to 2^-24 of the sum so far: 32 * 2^-24. The weights' two terms
+    are off by 2^-22, the warps' or CTAs' merge, the division and its product by eight roundings of 2^-24."""
+    p = Problem(kv, b, s, h, kvh, d, n, [0] * b)
+    p.past[:] = n - s
+    third = torch.tensor(1 / 3, device="cuda")
+    top = 127 if kv == "int8" else 448
+    p.rows[:, : h * d] = 1.0
+    p.rows[:, h * d: (h + kvh) * d] = 0
+    p.rows[:, (h + kvh) * d:] = third * top
+    p.codes[0].zero_()
+    p.scales[0].fill_(1.0)
+    p.codes[1].fill_(127 if kv == "int8" else 0x7e)
+    p.scales[1].fill_(third)
+    p.attend(ctx)
+    want = float(third) * top
+    bound = 32 * 2.0 ** -23 + 32 * 2.0 ** -24 + 2.0 ** -22 + 8 * 2.0 ** -24
+    assert float((p.out.double() / want - 1).abs().max()) <= bound
