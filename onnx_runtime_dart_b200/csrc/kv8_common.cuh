@@ -589,7 +589,9 @@ __device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int
 #pragma unroll
   for (int u = 0; u < NC; u++)
     o.v[u] = make_float4(o.v[u].x * f1 * f2, o.v[u].y * f1 * f2, o.v[u].z * f1 * f2, o.v[u].w * f1 * f2);
-  o.factor = a.scale * LOG2E / f1 / f2;
+  // Never 0 (a row of zeros under a scale below 2^-12 would come to less than the
+  // smallest number): hidden scores are -inf before they are multiplied.
+  o.factor = fmaxf(a.scale * LOG2E / f1 / f2, __uint_as_float(1u));
   o.lim = !valid ? -1 : (a.tree ? past - 1 : past + i);
   o.bits = valid && a.tree ? a.tree[(int64_t)b * a.S + i] : 0;
 }

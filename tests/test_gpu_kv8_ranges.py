@@ -183,3 +183,16 @@ def test_sums_do_not_drift(ctx, kv, b, s, h, kvh, d, n):
     want = float(third) * top
     bound = 32 * 2.0 ** -23 + 32 * 2.0 ** -24 + 2.0 ** -22 + 8 * 2.0 ** -24
     assert float((p.out.double() / want - 1).abs().max()) <= bound
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("s,d", [(3, 128), (60, 128), (64, 64), (5, 80)])
+@pytest.mark.parametrize("scale", [1.0, 1e-3, 1e-6, 1e-20, 1e-37])
+def test_zero_queries_under_a_small_scale(ctx, s, d, scale, tree):
+    """Rows of zeros among the queries weigh all they see alike, whatever the scale; hidden keys stay hidden."""
+    p = Problem("int8", 2, s, 4, 2, d, 200, [90, 0], scale=scale, tree=_random_tree(2, s, 3) if tree else None)
+    p.rows[::2, : 4 * d] = 0
+    p.rows[1::2, : 4 * d] *= 1e-38  # subnormal and nearly so
+    p.attend(ctx)
+    want, tol, _ = p.answer()
+    assert bool(((p.out.double() - want).abs() <= tol).all())
