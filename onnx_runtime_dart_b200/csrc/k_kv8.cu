@@ -173,7 +173,7 @@ template <bool E4M3>
 __global__ void __launch_bounds__(256) kv8_attend_kernel(const Kv8Args a) {
   pdl_launch_dependents();
   __shared__ float qs[256], wo[8][256], wm[8], wl[8];
-  __shared__ float sums[8];
+  __shared__ double sums[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int kvh = h / (a.H / a.KVH), D = a.D;
@@ -181,15 +181,12 @@ __global__ void __launch_bounds__(256) kv8_attend_kernel(const Kv8Args a) {
   const int64_t pos = token_pos(a, b, i, past);
   float x = tid < D ? a.q[((int64_t)b * a.S + i) * a.q_rs + (int64_t)h * D + tid] : 0.f;
   if (a.q_gain) {
-    float ss = x * x;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const double ss = warp_sum_d((double)x * x);
     if (lane == 0) sums[warp] = ss;
     __syncthreads();
     double t = 0.0;
     for (int w = 0; w < 8; w++) t += sums[w];
-    const float inv = (float)(1.0 / sqrt(t / D + a.eps));
-    if (tid < D) x = x * inv * a.q_gain[(int64_t)h * D + tid];
+    if (tid < D) x = (float)((double)x * (1.0 / sqrt(t / D + a.eps)) * a.q_gain[(int64_t)h * D + tid]);
   }
   qs[tid] = x;
   __syncthreads();

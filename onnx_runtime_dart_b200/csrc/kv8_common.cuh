@@ -515,15 +515,28 @@ __device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int
       n4[u] = *reinterpret_cast<const float4 *>(a.sin + at);
     }
   }
-  float inv = 1.f;
+  float inv = 1.f, pre = 1.f;
   if (gain) {
-    float ss = 0.f;
+    auto squares = [&]() {
+      float ss = 0.f;
 #pragma unroll
-    for (int u = 0; u < NC; u++)
-      ss = fmaf(o.v[u].x, o.v[u].x, fmaf(o.v[u].y, o.v[u].y, fmaf(o.v[u].z, o.v[u].z, fmaf(o.v[u].w, o.v[u].w, ss))));
+      for (int u = 0; u < NC; u++)
+        ss = fmaf(o.v[u].x, o.v[u].x, fmaf(o.v[u].y, o.v[u].y, fmaf(o.v[u].z, o.v[u].z, fmaf(o.v[u].w, o.v[u].w, ss))));
 #pragma unroll
-    for (int f = 1; f < 8; f <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, f);
+      for (int f = 1; f < 8; f <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, f);
+      return ss;
+    };
+    float ss = squares();
     inv = 1.f / sqrtf(ss / D + (float)a.eps);
+    // Rows whose squares leave fp32's comfortable range are first brought near 1.
+    const bool wide = !(ss > 1e-30f && ss < 1e36f);
+    if (__any_sync(0xffffffffu, wide)) {
+      if (wide) pre = ss > 1.f ? 0x1p-100f : 0x1p100f;
+#pragma unroll
+      for (int u = 0; u < NC; u++) o.v[u].x *= pre, o.v[u].y *= pre, o.v[u].z *= pre, o.v[u].w *= pre;
+      ss = squares();
+      if (wide) inv = (float)(1.0 / sqrt((double)ss / D + a.eps * pre * pre));
+    }
   }
   if (gain) {
 #pragma unroll
@@ -561,7 +574,8 @@ __device__ __forceinline__ void load_q_row(const Kv8Args &a, int b, int kvh, int
         float4 w4 = *reinterpret_cast<const float4 *>(src + e);
         if (gain) {
           const float4 g4 = *reinterpret_cast<const float4 *>(gain + e);
-          w4.x *= inv * g4.x, w4.y *= inv * g4.y, w4.z *= inv * g4.z, w4.w *= inv * g4.w;
+          w4.x = w4.x * pre * (inv * g4.x), w4.y = w4.y * pre * (inv * g4.y);
+          w4.z = w4.z * pre * (inv * g4.z), w4.w = w4.w * pre * (inv * g4.w);
         }
         c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w;
         const float sg = first ? 1.f : -1.f;

@@ -196,3 +196,16 @@ def test_zero_queries_under_a_small_scale(ctx, s, d, scale, tree):
     p.attend(ctx)
     want, tol, _ = p.answer()
     assert bool(((p.out.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("e", [62, 70, 120, -60, -100])
+@pytest.mark.parametrize("s,d,rot,inter", [(1, 128, 128, False), (3, 64, 32, False), (2, 96, 96, True), (70, 128, 64, False),
+                                           (90, 64, 64, False), (2, 80, 80, False), (1, 256, 0, False)])
+def test_head_norm_of_large_and_small_queries(ctx, s, d, rot, inter, e):
+    """Queries whose squares leave fp32's range are normalised all the same (one row in three stays as it is)."""
+    p = Problem("int8", 2, s, 4, 2, d, 200, [90, 7], rot, inter, True, half=d // 2)
+    r = p.rows.view(2 * s, 8, d)
+    r[:, [0, 1, 3]] *= 2.0 ** e
+    p.attend(ctx)
+    want, tol, _ = p.answer()
+    assert bool(((p.out.double() - want).abs() <= tol).all())
