@@ -168,8 +168,10 @@ struct Scratch {
     if (need == 0) return;
     cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
     B2M_CUDA(cudaStreamIsCapturing(ctx->stream, &cs));
+    const bool capturing = cs == cudaStreamCaptureStatusActive;
     if (need > ctx->scratch_bytes) {
-      if (ctx->scratch && ctx->scratch_in_graph)
+      // (during a capture work that was enqueued before may still use it, too)
+      if (ctx->scratch && (ctx->scratch_in_graph || capturing))
         ctx->retired_scratch.push_back(ctx->scratch);
       else if (ctx->scratch)
         B2M_CUDA(cudaFreeAsync(ctx->scratch, ctx->stream));
@@ -177,10 +179,20 @@ struct Scratch {
       ctx->scratch_bytes = 0;
       ctx->scratch_in_graph = false;
       const size_t sz = std::max(need, (size_t)1 << 20);
-      B2M_CUDA(cudaMallocAsync(&ctx->scratch, sz, ctx->stream));
+      if (capturing) {
+        // A stream-ordered allocation would become a node of the graph, with memory
+        // that is there only while the graph runs; later calls use it outside.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        B2M_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        const cudaError_t e = cudaMalloc(&ctx->scratch, sz);
+        B2M_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        B2M_CUDA(e);
+      } else {
+        B2M_CUDA(cudaMallocAsync(&ctx->scratch, sz, ctx->stream));
+      }
       ctx->scratch_bytes = sz;
     }
-    if (cs == cudaStreamCaptureStatusActive) ctx->scratch_in_graph = true;
+    if (capturing) ctx->scratch_in_graph = true;
   }
   void *take(size_t bytes) {
     const size_t off = (used + 255) & ~(size_t)255;
@@ -796,9 +808,8 @@ B2M_API b2m_status b2m_shutdown(b2m_ctx *ctx) {
     DeviceGuard dg(ctx->device);
     cudaStreamSynchronize(ctx->stream);
     cudaStreamSynchronize(ctx->own_stream);
-    if (ctx->scratch) cudaFreeAsync(ctx->scratch, ctx->own_stream);
-    for (void *p : ctx->retired_scratch) cudaFreeAsync(p, ctx->own_stream);
-    cudaStreamSynchronize(ctx->own_stream);
+    if (ctx->scratch) cudaFree(ctx->scratch);  // (of either allocator)
+    for (void *p : ctx->retired_scratch) cudaFree(p);
     if (ctx->pinned) cudaFreeHost(ctx->pinned);
     if (ctx->err_host) cudaFreeHost(ctx->err_host);
     cudaFree(ctx->dev_counter);

@@ -1,5 +1,6 @@
 """GPU tests of the context's workspace and CUDA graphs: a graph keeps the
-workspace it was captured on."""
+workspace it was captured on, and one that a capture has to enlarge serves the
+calls outside the graph as well."""
 import ctypes
 
 import numpy as np
@@ -75,6 +76,45 @@ def test_a_graph_keeps_a_workspace_that_was_replaced():
     del g
     op.close()
     other.close()
+
+
+def test_a_capture_enlarges_the_workspace():
+    """The first call of a context, and a larger one later, under a capture: the same rows as an uncaptured call's, from
+    the graphs in any order and from calls outside them."""
+    plain, op = Gemm(), Gemm()
+    small, large, huge = _rows(300, 3), _rows(1500, 4), _rows(5000, 5)
+    want = []
+    for x, y in (small, large, huge):
+        plain(x, y)
+        torch.cuda.synchronize()
+        want.append(y.clone())
+    g0 = _capture(lambda: op(*small))
+    op(*small)                       # outside the graph, before it ever ran
+    torch.cuda.synchronize()
+    assert torch.equal(small[1], want[0])
+    g1 = _capture(lambda: op(*large))
+    graphs = {0: g0, 1: g1}
+    for k in (1, 0, 1, 0, 0, 1):
+        y = (small, large)[k][1]
+        y.zero_()
+        graphs[k].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[k])
+        op(*(small, large)[1 - k])
+        torch.cuda.synchronize()
+        assert torch.equal((small, large)[1 - k][1], want[1 - k])
+    op(*huge)                        # and one that replaces what the second graph holds
+    torch.cuda.synchronize()
+    assert torch.equal(huge[1], want[2])
+    for k in (0, 1):
+        y = (small, large)[k][1]
+        y.zero_()
+        graphs[k].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[k])
+    del g0, g1, graphs
+    op.close()
+    plain.close()
 
 
 def test_a_wide_verify_between_replays_of_the_decode_step():
