@@ -566,13 +566,13 @@ B2M_API b2m_status b2m_kv8_read_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, co
  * and the new tokens j whose bit j is set (a token sees itself only if its
  * own bit is set; one that sees nothing gets zeros). out: [b][s] rows of
  * h*head_dim, and / or out16, the same rounded to f16 (h*head_dim % 8 == 0);
- * one of them may be NULL. Scale <= 0 means 1/sqrt(head_dim). A token's result
- * keeps its digits whatever the value rows that it does not see, or hardly
- * weighs, hold, as long as they are below 2^85 times those that it does. The queries
- * and the softmax weights are split into two f16 terms on the tensor cores
- * (about 1e-6 of the largest value of a row, however many keys it sees);
- * out16 holds the same rows rounded once, with or without out. EXACT attention mode (b2m_set_attention_mode) runs
- * the fp32 CUDA-core kernel. */
+ * one of them may be NULL. Scale <= 0 means 1/sqrt(head_dim). The queries and
+ * the softmax weights are split into two f16 terms on the tensor cores (about
+ * 1e-6 of the largest value of a row, however many keys it sees); out16 holds the
+ * same rows rounded once, with or without out. A token's result keeps its digits
+ * whatever the value rows that it does not see, or hardly weighs, hold, as long as
+ * they are below 2^85 times those that it does. EXACT attention mode
+ * (b2m_set_attention_mode) runs the fp32 CUDA-core kernel. */
 B2M_API b2m_status b2m_gqa_kv8_dev(b2m_ctx *ctx, const b2m_kv8_cache *cache, const float *q, const float *k,
                                    const float *v, int64_t q_rs, int64_t kv_rs, const float *qk_gain, double eps,
                                    const int32_t *past, const uint64_t *tree, const int32_t *depth,

@@ -29,12 +29,13 @@
 // split the keys and merge their O, reference and l through distributed shared memory in
 // rank order; no workspace, no atomics.
 //
-// 4 x 2048 causal tokens (16 heads on 8) take 235 us with their append: 292 TFLOP/s
-// of wanted products, tensor pipe 25% busy (P's second term included), issue slots
-// 52%. What bounds it is the instructions of the softmax and of the expansion (some
-// 4500 per 64-key tile and CTA) and each CTA's start and end, which only the SM's
-// other CTA covers (query rows loaded by all warps ahead of the tiles, and rows
-// stored one at a time: 245 us).
+// 4 x 2048 causal tokens (16 heads on 8) take 275 us with their append: 250 TFLOP/s
+// of wanted products, tensor pipe 29% busy (second terms included), issue slots 46%.
+// What bounds it is the instructions of the softmax and of the expansion (some
+// 4500 per 64-key tile and CTA), the single K and V tile, and each CTA's start, totals
+// and end, which only the SM's other CTA covers. 237 us were without the second term
+// of Q, whose room held another tile of each, and without the totals; 257 without the
+// totals alone.
 //
 // Every wait is bounded; one that gives up records the device error and all
 // roles leave their loops.
@@ -462,8 +463,8 @@ __global__ void __launch_bounds__(FL_THREADS, 2) kv8_flash_kernel(const Kv8Args 
     // zero: eight times per tile, 1.6e-7 of a sum of equal signs (1e-5 after 60 tiles,
     // without a bound as sequences grow). So O starts anew every FL_WINDOW tiles, and
     // the row's thread adds what it held, rounded to nearest, to totals of its own:
-    // thread-local memory, which is laid out across a warp's threads and mostly stays
-    // in L2. `carry` is what the totals are to be multiplied by since the last time.
+    // thread-local memory, which is laid out across a warp's threads and stays in L2 (the
+    // driver keeps 190 MB of it for the device). `carry` is what the totals are to be multiplied by since the last time.
     alignas(16) float total[D];
     float carry = 1.f;
     // Waits for phase `parity` of `done`, then calls put(d, totals + O of dimensions d ..
@@ -773,7 +774,8 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   const int nrows = a.S * (a.H / a.KVH), tiles = (nrows + FL_ROWS - 1) / FL_ROWS;
   // Key splits up to one wave (two CTAs per SM), each with two tiles or more; and
   // two for calls of one to two waves over a long cache, whose second wave would
-  // be part empty (400 CTAs of 59 tiles: 276 us, 308 unsplit, 322 with four).
+  // be part empty (400 CTAs of 59 tiles: 283 us, 326 unsplit, 321 with four; a causal
+  // call from an empty cache, 512 CTAs of 1 to 32 tiles, loses: 179 us, 153 unsplit).
   const int64_t ctas = (int64_t)a.B * a.KVH * tiles, wave = 2 * (int64_t)device_sm_count();
   int cl = 1;
   while (cl < FL_MAX_CLUSTER && ctas * cl * 2 <= wave && a.CAP > 2 * FL_TILE * cl) cl *= 2;
@@ -798,10 +800,11 @@ void launch(const Kv8Args &a, cudaStream_t s) {
 }  // namespace
 
 // Enough rows, head dims and alignments the kernel takes. The other kernel reads
-// the cache once per 16 rows: above 48 rows this one is faster however few CTAs
-// there are, from 33 on where the other's CTAs are more than one wave (32 x 8
-// (sequence, kv head)s over 1500 keys: 40 rows 74 us, 99 there, 48 rows 75 and 100;
-// 32 rows 72 and 69. With 2 x 8 over 6000 keys 48 rows take 45 and 37).
+// the cache once per 16 rows: from 33 rows on this one is faster where the other's
+// CTAs are more than one wave (32 x 8 (sequence, kv head)s over 1500 keys: 40 rows
+// 98 us, 137 there, 48 rows 99 and 139; 32 rows 98 and 97). With few CTAs it takes over
+// from 49 rows (2 x 8 over 6000 keys: 48 rows 53 us, 45 there, 64 rows 54 and 46: the
+// border lies higher still).
 bool kv8_flash_shape(const Kv8Args &a) {
   auto al = [](const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   const int64_t rows = (int64_t)a.S * (a.H / a.KVH);

@@ -10,19 +10,19 @@
 // they are expanded in registers and the scales applied in fp32, K's to the
 // scores and V's to the weights. Q and the weights are split into two f16 terms (22
 // bits), so the products carry fp32 accuracy, for an f16 output too (one term of the
-// weights would put 2.9e-4 of error where the output's own rounding is 2.1e-4). Which D index or key an MMA
-// lane holds is free as long as both operands agree: lanes are given 16
-// consecutive bytes of a row, so no data is shuffled on its way to the tensor
+// weights would put 2.9e-4 of error where the output's own rounding is 2.1e-4). Which
+// D index or key an MMA lane holds is free as long as both operands agree: lanes are
+// given 16 consecutive bytes of a row, so no data is shuffled on its way to the tensor
 // cores; only P^T is transposed between the two products (movmatrix).
 //
 // Should be bound by HBM (2 D + 8 bytes per key of a kv head): 64 sequences over
-// 4096 .. 8191 positions of 8 kv heads take 168 us, 4.98 TB/s (floor 129); the warps'
+// 4096 .. 8191 positions of 8 kv heads take 176 us, 4.8 TB/s (floor 129); the warps'
 // own chains (expand, product, exp2, product) and the part-empty last wave are the
-// rest, issue slots 49% used. Each lane copies the bytes it will use itself into a
+// rest, issue slots 50% used. Each lane copies the bytes it will use itself into a
 // ring of its own in shared memory (cp.async), two tiles ahead, so that enough
-// loads are in flight without registers and no barrier is needed in the loop (one
-// tile ahead 184 us, three 169; four CTAs per SM instead of three 184, six warps
-// per CTA 185, eight 223).
+// loads are in flight without registers and no barrier is needed in the loop (when
+// all took 168 us: one tile ahead 184, three 169; four CTAs per SM instead of three
+// 184, six warps per CTA 185, eight 223).
 //
 // V scales are taken relative to the largest the warp has met (a power of two). A
 // row's softmax reference goes by its own largest weight times V scale (weight_ref)
@@ -96,7 +96,7 @@ struct StepSmem {
 };
 
 // (The CTAs per SM that the registers allow anyway, said to the compiler: 32 trees
-// of 8 tokens 42 us, 45 .. 47 without.)
+// of 8 tokens 42 us, 45 .. 47 without; 48 with the totals of ST_WINDOW.)
 template <bool E4M3, int D, int NT>
 __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? (NT == 1 ? 3 : 2) : 1)
     kv8_step_kernel(const Kv8Args a, const int fused_append) {
@@ -555,10 +555,10 @@ void launch(const Kv8Args &a, cudaStream_t s) {
   // wave of CTAs that are resident together (three per SM for 8 query rows, two for
   // 16), at least 128 cache positions each, 16 CTAs at most; and two for calls of
   // between one and two waves of long rows, whose second wave would be mostly
-  // empty (measured before the last steps, 64 sequences over 4096 .. 8191 positions:
-  // 179 us, 208 unsplit; 32 trees over 1500: 45 us unsplit, 61 and 66 with two and
+  // empty (64 sequences over 4096 .. 8191 positions: 176 us, 207
+  // unsplit, 202 with four; 32 trees over 1500: 48 us unsplit, 51 and 70 with two and
   // four). Three sequences over 40000 (12 x 16 CTAs) are bound by the SMs that hold
-  // two CTAs: 40 us; clusters of 8, 9, 12 and 14: 50, 46, 50, 44.
+  // two CTAs: 41 us; clusters of 8 and 4: 52 and 94.
   const int64_t ctas = (int64_t)a.B * a.KVH * tiles;
   const int64_t wave = (NT == 1 ? 3 : 2) * (int64_t)b2m::device_sm_count();
   int cl = 1;
