@@ -209,3 +209,61 @@ def test_head_norm_of_large_and_small_queries(ctx, s, d, rot, inter, e):
     p.attend(ctx)
     want, tol, _ = p.answer()
     assert bool(((p.out.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+@pytest.mark.parametrize("seed", range(12))
+def test_values_of_any_size(ctx, kv, seed):
+    """Value rows of random magnitudes, 2^-20 .. 2^20 from one key to the next and some of zeros, over random shapes."""
+    g = torch.Generator().manual_seed(seed)
+
+    def pick(*xs):
+        return xs[int(torch.randint(0, len(xs), (1,), generator=g))]
+
+    d, kvh = pick(32, 64, 64, 96, 128, 128, 256, 80), pick(1, 2, 4)
+    h, s = kvh * pick(1, 2, 3, 8), pick(1, 1, 2, 7, 30, 64, 200)
+    b, past = pick(1, 2, 5), pick(0, 5, 63, 300, 1500)
+    tree = _random_tree(b, s, seed, orphan=True) if s <= 64 and pick(True, False) else None
+    p = Problem(kv, b, s, h, kvh, d, past + s + pick(0, 9), [past] + [past // 2] * (b - 1), pick(0, d), False,
+                pick(True, False), tree=tree)
+    e = torch.randint(-20, 21, (b, kvh, past), generator=g).float()
+    e[torch.rand(e.shape, generator=g) < 0.1] = -math.inf
+    p.scales[1][:, :, :past] *= (2.0 ** e).cuda()
+    p.rows.view(b * s, -1, d)[:, h + kvh:] *= (2.0 ** torch.randint(-20, 21, (b * s, kvh, 1), generator=g).float()).cuda()
+    p.attend(ctx)
+    want, tol, _ = p.answer()
+    err, tol = (p.out.double() - want).abs(), _row_tol(p, tol)
+    assert bool((err <= tol).all()), f"{float((err / tol).max()):.2f} of the bound"
+
+
+@pytest.mark.parametrize("s,past", [(1, 300), (90, 1000), (1, 524000), (5, 524000), (150, 524000)])
+def test_offsets_beyond_32_bits(ctx, s, past):
+    """A cache of more than 2^32 bytes, the last sequence behind that border, with few and with many keys."""
+    b, kvh, d, cap = 9, 8, 128, 1 << 19
+    p = Problem("int8", b, s, kvh, kvh, d, 4, [0] * b)  # (its small cache is replaced)
+    free, _ = torch.cuda.mem_get_info()
+    if free < 20 << 30:
+        pytest.skip("needs 20 GB of device memory")
+    p.cap = cap
+    p.codes = [torch.zeros((b, kvh, cap, d), device="cuda", dtype=torch.uint8) for _ in range(2)]
+    p.scales = [torch.zeros((b, kvh, cap), device="cuda") for _ in range(2)]
+    g = torch.Generator(device="cuda").manual_seed(s)
+    for side in range(2):
+        p.codes[side][-1, :, :past] = torch.randint(0, 255, (kvh, past, d), generator=g, device="cuda",
+                                                    dtype=torch.uint8) + 129  # -127 .. 127
+        p.scales[side][-1, :, :past] = 0.01 + 0.01 * torch.rand((kvh, past), generator=g, device="cuda")
+    p.past[-1] = past
+    p.cache = N.Kv8Cache(p.codes[0].data_ptr(), p.codes[1].data_ptr(), p.scales[0].data_ptr(), p.scales[1].data_ptr(),
+                         N.B2M_INT8, b, kvh, cap, d)
+    p.attend(ctx)
+    new = p.new_rows()
+    for side in range(2):
+        assert torch.equal(_decode(p.codes[side][-1, :, past: past + s], "int8"), new[side][0][-1])
+    out = p.out
+    p.out = None
+    last = Problem("int8", 1, s, kvh, kvh, d, 4, [0])
+    last.rows, last.cap, last.past = p.rows[-s:], past + s, p.past[-1:]
+    last.codes = [t[-1:, :, : past + s] for t in p.codes]
+    last.scales = [t[-1:, :, : past + s] for t in p.scales]
+    want, tol, _ = last.answer()
+    assert bool(((out[-1:].double() - want).abs() <= tol).all())
